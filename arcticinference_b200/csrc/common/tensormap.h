@@ -44,10 +44,11 @@ inline int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
-// General N-D map (N <= 5), 128-byte swizzle. dims/box are innermost-first;
+// General N-D map (N <= 5), 128-byte swizzle unless said otherwise. dims/box are innermost-first;
 // strides_bytes has N-1 entries (dimension 0 is contiguous).
 inline int make_tmap_nd(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank,
-                        const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box) {
+                        const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                        CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn = get_encode_tiled();
   if (fn == nullptr) return -1;
   cuuint64_t d[5];
@@ -61,7 +62,7 @@ inline int make_tmap_nd(CUtensorMap* map, const void* base, CUtensorMapDataType 
     if (i + 1 < rank) s[i] = strides_bytes[i];
   }
   CUresult r = fn(map, dtype, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, e,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }

@@ -1,0 +1,484 @@
+// Products of microscaled 4-bit operands for sm_100a: out[m, n] = act(g_m h_n sum_b s_mb t_nb sum_{k in b} q_mk p_nk
+// + bias_n) + residual_mn, tokens m, features n, blocks b of 16 (nvfp4) or 32 (mxfp4) columns; one matrix, or each row
+// with its expert's (rows sorted by expert, the list of row tiles made on the device by the router).
+//
+// tcgen05.mma kind::mxf4nvf4 / mxf4 takes the blocks' scales from tensor memory and multiplies e2m1 codes at twice the
+// rate of fp8; the fp32 accumulator needs no rescaling, only the factors of rows and features at the end.
+//
+// Features are the tensor core's M side (128 per CTA), tokens its N side: a step's instruction is as wide as
+// there are tokens, so a single token or a ragged group costs what it has. One thread feeds a ring of stages by TMA:
+// 256 columns of both operands (128 bytes a row, 128-byte swizzle) and their scale tiles. One warp copies a stage's
+// scales to tensor memory (two sets, used in turn) and issues the products into one of two accumulators;
+// eight warps drain the other one. A lane then holds one feature of many tokens: four lanes exchange four by four
+// values and store eight bytes, 64 consecutive bytes per token and instruction.
+
+#include <string.h>
+
+#include "api.h"
+#include "common/elem.cuh"
+#include "common/fp4.cuh"
+#include "common/pdl.cuh"
+#include "common/tensormap.h"
+
+namespace ab200 {
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int kF4EpilogueWarps = 8;
+constexpr int kF4Threads = (2 + kF4EpilogueWarps) * 32;
+constexpr int kF4MaxStages = 10;
+constexpr int kF4StepCols = 256;                       // columns of a stage: 128 bytes of codes
+constexpr uint32_t kF4ABytes = 128 * 128;
+constexpr uint32_t kF4ScaleAt = 384;                   // tensor memory: accumulators at 0 and 192, then two sets of scales
+constexpr uint32_t kF4ScaleSet = 64;
+constexpr int kF4MaxTokens = 192;
+
+struct Fp4GemmArgs {
+  int N, M, kblocks, n_tiles, m_tiles;
+  int bn;                  // tokens of a tile
+  int stages;
+  uint32_t b_bytes, sfa_bytes, sfb_bytes;
+  int sfb_tiles;           // row tiles that the scales of a tile's tokens lie in
+  int w_row_tiles;         // row tiles of scales per matrix
+  int act, has_gate;
+  GateParams gate;
+  const int4* tiles;
+  const int* num_tiles;
+  const float* x_scale;    // nvfp4: factor per token, null: 1
+  const float* w_scale;    // factor per feature [groups][N], null: 1
+  const bf16* bias;
+  const bf16* residual;
+  long long ldr;
+  bf16* out;
+  long long ldo;
+  int* status;
+};
+
+struct F4Work {
+  int nt;                  // feature tile
+  int group, row0, nrows;  // matrix, first token, tokens
+  int slot;                // row tile of the tokens' scales
+  int shift;               // first token's place in it, in columns of 32
+};
+
+template <bool PAIR>
+__device__ __forceinline__ F4Work f4_work(const Fp4GemmArgs& p, int w) {
+  F4Work r;
+  if (p.tiles != nullptr) {
+    r.nt = w % p.n_tiles;
+    const int mt = w / p.n_tiles;
+    const int4 t = p.tiles[mt];
+    r.group = t.x;
+    r.row0 = t.y;
+    r.nrows = t.z;
+    r.slot = mt;
+    r.shift = 0;
+    return r;
+  }
+  // groups of eight feature tiles: what the resident CTAs read stays in L2
+  const int per = 8 * p.m_tiles, first = w / per * 8;
+  const int wide = min(8, p.n_tiles - first), in = w % per;
+  r.nt = first + in % wide;
+  const int mt = in / wide;
+  r.group = 0;
+  r.row0 = mt * p.bn;
+  r.nrows = min(p.bn, p.M - r.row0);
+  r.slot = r.row0 / kFp4TileRows;
+  r.shift = r.row0 % kFp4TileRows / 32;
+  return r;
+}
+
+// Columns of the instruction: what a tile has, in steps of 16
+__device__ __forceinline__ int f4_width(int nrows) { return (nrows + 15) & ~15; }
+
+__device__ __forceinline__ float gelu_exact(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752f)); }
+
+__device__ __forceinline__ float f4_gated(int act, const GateParams& p, float g, float u) {
+  float t;   // g * sigmoid(t)
+  if (act == kActClampedSwish) {
+    g = fminf(g, p.limit);
+    u = fminf(fmaxf(u, -p.limit), p.limit) + 1.f;
+    t = p.alpha * g;
+  } else {
+    t = act == kActSilu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+  }
+  return __fdividef(g, 1.f + __expf(-t)) * u;
+}
+
+// v[i]: token i's value of this lane's feature; afterwards lane 4 a + q has token q's features 4 a .. 4 a + 3.
+__device__ __forceinline__ void f4_transpose4(float (&v)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+  float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
+  float s1 = __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
+  const float a0 = odd ? s0 : v[0], a1 = odd ? v[1] : s0;     // token 0 or 1: features f, f + 1
+  const float b0 = odd ? s1 : v[2], b1 = odd ? v[3] : s1;     // token 2 or 3
+  s0 = __shfl_xor_sync(0xffffffffu, high ? a0 : b0, 2);
+  s1 = __shfl_xor_sync(0xffffffffu, high ? a1 : b1, 2);
+  v[0] = high ? s0 : a0;
+  v[1] = high ? s1 : a1;
+  v[2] = high ? b0 : s0;
+  v[3] = high ? b1 : s1;
+}
+
+// 32 tokens from c0 on of a finished tile; the lane's feature is feature0 + lane. cols: the tokens' factors.
+__device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t (&r)[32], const float* cols, int c0,
+                                           int row0, int nrows, int feature0, float h, float bias, int lane) {
+  if (p.has_gate) {
+    // lanes 0 - 15: gate rows, 16 - 31 their up rows. The lower half joins the even tokens, the upper the odd ones.
+    const int f = (feature0 >> 1) + (lane & 12);
+    const bool up = lane >= 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = 8 * i + 2 * j;
+        const float2 g = *reinterpret_cast<const float2*>(cols + t);
+        const float even = __uint_as_float(r[t]) * (g.x * h), odd = __uint_as_float(r[t + 1]) * (g.y * h);
+        const float other = __shfl_xor_sync(0xffffffffu, up ? even : odd, 16);
+        v[j] = f4_gated(p.act, p.gate, up ? other : even, up ? odd : other);
+      }
+      f4_transpose4(v, lane);
+      const int t = c0 + 8 * i + 2 * (lane & 3) + (up ? 1 : 0);
+      if (t < nrows && 2 * f < p.N)
+        store4(p.out + (long long)(row0 + t) * p.ldo + f, make_float4(v[0], v[1], v[2], v[3]));
+    }
+    return;
+  }
+  const int f = feature0 + (lane & ~3);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (c0 + 4 * i >= nrows) break;
+    const float4 g = *reinterpret_cast<const float4*>(cols + 4 * i);
+    float v[4] = {__uint_as_float(r[4 * i]) * (g.x * h) + bias, __uint_as_float(r[4 * i + 1]) * (g.y * h) + bias,
+                  __uint_as_float(r[4 * i + 2]) * (g.z * h) + bias, __uint_as_float(r[4 * i + 3]) * (g.w * h) + bias};
+    if (p.act == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = gelu_exact(v[j]);
+    }
+    f4_transpose4(v, lane);
+    const int t = c0 + 4 * i + (lane & 3);
+    if (t < nrows && f < p.N) {
+      const long long row = row0 + t;
+      if (p.residual != nullptr) {
+        const float4 a = load4(p.residual + row * p.ldr + f);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      }
+      store4(p.out + row * p.ldo + f, make_float4(v[0], v[1], v[2], v[3]));
+    }
+  }
+}
+
+template <bool MX>
+__global__ void __launch_bounds__(kF4Threads, 1)
+fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
+                const Fp4GemmArgs p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
+    pdl_trigger();
+    pdl_wait();
+    if (threadIdx.x == 0) report_error(p.status, kErrBadArgument, 1500, (int)(smem_u32(smem) & 1023u));
+    return;
+  }
+  const uint32_t stage_bytes = kF4ABytes + p.b_bytes + p.sfa_bytes + p.sfb_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * stage_bytes);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kF4MaxStages + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* cols = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);   // 32 floats a warp
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bars_base = smem_u32(bars);
+  auto full_bar = [&](int s) { return bars_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bars_base + 8u * (kF4MaxStages + s); };
+  auto tfull_bar = [&](int a) { return bars_base + 8u * (2 * kF4MaxStages + a); };
+  auto tempty_bar = [&](int a) { return bars_base + 8u * (2 * kF4MaxStages + 2 + a); };
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), kF4EpilogueWarps);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&tmap_w);
+    prefetch_tensormap(&tmap_x);
+    prefetch_tensormap(&tmap_sw);
+    prefetch_tensormap(&tmap_sx);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();   // (tensor memory is owned)
+  pdl_wait();
+  const int total_work = (p.tiles != nullptr ? *p.num_tiles : p.m_tiles) * p.n_tiles;
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < total_work && ok; w += gridDim.x) {
+        const F4Work t = f4_work<false>(p, w);
+        if (t.nrows <= 0) continue;
+        const int feature0 = t.nt * 128;
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 1500 + stage, kb)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
+          const uint32_t dst = smem_base + (uint32_t)stage * stage_bytes;
+          const uint32_t sfa = dst + kF4ABytes + p.b_bytes;
+          constexpr int kTiles = MX ? 2 : 4;
+          tma_load_3d(dst, &tmap_w, full_bar(stage), kb * 128, feature0, t.group);
+          tma_load_2d(dst + kF4ABytes, &tmap_x, full_bar(stage), kb * 128, t.row0);
+          tma_load_3d(sfa, &tmap_sw, full_bar(stage), 0, kb * kTiles, t.group * p.w_row_tiles + t.nt);
+          tma_load_3d(sfa + p.sfa_bytes, &tmap_sx, full_bar(stage), 0, kb * kTiles, t.slot);
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {   // copies already issued get a short time to land
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 20000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer -------------------------------
+    // (uniform control and one elected lane, see gemm_bf16.cu)
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
+    const uint64_t a0 = make_desc_kmajor_sw128(smem_base);
+    const uint64_t s0 = make_desc_scales(smem_base + kF4ABytes + p.b_bytes);
+    const uint64_t stage_step = stage_bytes / 16;
+    const uint32_t sfb_cols = 4u * (uint32_t)p.sfb_tiles;
+    constexpr int kTiles = MX ? 2 : 4;
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    // the stages of the last step and of the one before: its products must be done before its set of scales is
+    // written again
+    int last_stage = -1, old_stage = -1;
+    uint32_t last_phase = 0, old_phase = 0, set = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; w < total_work && ok; w += gridDim.x) {
+      const F4Work t = f4_work<false>(p, w);
+      if (t.nrows <= 0) continue;
+      if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.status,
+                                             1600 + acc, w)))
+        break;
+      tc_fence_after();
+      const uint32_t n = (uint32_t)f4_width(t.nrows);
+      const uint32_t idesc = make_idesc_fp4(128, n, MX, 0), idesc_hi = make_idesc_fp4(128, n, MX, 2);
+      const uint32_t d_tmem = tm + (uint32_t)acc * (uint32_t)kF4MaxTokens;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (old_stage >= 0 && !__all_sync(0xffffffffu, mbar_wait(empty_bar(old_stage), old_phase, abort_flag,
+                                                                 p.status, 1620 + stage, kb))) {
+          ok = false;
+          break;
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.status, 1640 + stage, kb))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t a_desc = a0 + (uint64_t)stage * stage_step;
+        const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
+        const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
+        const uint64_t sb_desc = sa_desc + (uint64_t)(p.sfa_bytes / 16);
+        const uint32_t sfa = tm + kF4ScaleAt + set * kF4ScaleSet, sfb = sfa + 16u;
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+            tmem_copy_scales<false>(sfa + 4u * j, sa_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
+            for (int i = 0; i < p.sfb_tiles; ++i)
+              tmem_copy_scales<false>(sfb + sfb_cols * j + 4u * i,
+                                      sb_desc + (uint64_t)((i * kTiles + j) * (kFp4ScaleTile / 16)));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int j = MX ? k / 2 : k;
+            umma_fp4_ss<MX, false>(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
+                                   MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j,
+                                   sfb + sfb_cols * j + (uint32_t)t.shift, (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit(empty_bar(stage));
+          if (kb == p.kblocks - 1) tc_commit(tfull_bar(acc));
+        }
+        __syncwarp();
+        old_stage = last_stage;
+        old_phase = last_phase;
+        last_stage = stage;
+        last_phase = phase;
+        set ^= 1u;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  } else {
+    // --------------------------------- epilogue --------------------------------
+    const int quad = warp & 3;            // TMEM lane quadrant this warp may read
+    const int half = (warp - 2) >> 2;     // which of the quadrant's two warps this is
+    float* my_cols = cols + (warp - 2) * 32;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int w = blockIdx.x; w < total_work; w += gridDim.x) {
+      const F4Work t = f4_work<false>(p, w);
+      if (t.nrows <= 0) continue;
+      const int feature0 = t.nt * 128 + quad * 32;
+      const int f = min(feature0 + lane, p.N - 1);
+      const float h = p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f;
+      const float bias = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 1700 + acc, w)))
+        break;
+      tc_fence_after();
+      const uint32_t t_addr = tmem_base + (uint32_t)acc * (uint32_t)kF4MaxTokens + ((uint32_t)(quad * 32) << 16);
+      for (int c0 = 32 * half; c0 < t.nrows && feature0 < p.N; c0 += 64) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_x32(t_addr + (uint32_t)c0, r);
+        my_cols[lane] = p.x_scale != nullptr && c0 + lane < t.nrows ? p.x_scale[t.row0 + c0 + lane] : 1.f;
+        __syncwarp();
+        tmem_ld_wait_dep(r);
+        f4_store32(p, r, my_cols, c0, t.row0, t.nrows, feature0, h, bias, lane);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty_bar(acc));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace ab200
+
+using namespace ab200;
+
+extern "C" {
+
+// x: codes [M, K / 2] (rows ldx bytes apart), scale tiles sx [row tiles][k_tiles][512], factors gx fp32 [M] or null;
+// w: codes [groups][N][K / 2] (w_gstride and ldw bytes), scale tiles sw [groups][ceil(N / 128)][k_tiles][512], factors
+// gw fp32 [groups][N] or null; out bf16. K a multiple of 32, N of 8 (of 32 with a gate), strides of codes multiples of
+// 16 bytes, ldo and ldr of 8 elements. fmt: 0 nvfp4, 1 mxfp4. act: 0, 1 (GELU); gate: 0, 1 (silu), 2 (gelu_tanh), 3
+// (clamped swish): rows of w alternate 16 gate and 16 up rows and out has N / 2 columns. With `tiles` (int32 x 4:
+// group, first row, rows; *num_tiles of them, at most max_tiles) row tile i's scales are sx's i-th row tile.
+int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* gx, const void* w, long long ldw,
+                     long long w_gstride, const void* sw, const void* gw, void* out, long long ldo, long long M,
+                     int N, int K, int groups, int fmt, const void* bias, const void* residual, long long ldr, int act,
+                     int gate, float gate_limit, float gate_alpha, const void* tiles, const void* num_tiles,
+                     int max_tiles, int* status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || groups <= 0 || (tiles != nullptr && max_tiles <= 0)) return 0;
+  auto odd = [](const void* q, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(q) & mask) != 0; };
+  if ((K % 32) || (N % 8) || (gate != 0 && N % 32) || gate < 0 || gate > 3 || act < 0 || act > 1 || fmt < 0 || fmt > 1 ||
+      (ldx % 16) || (ldw % 16) || (w_gstride % 16) || (ldo % 8) || (ldr % 8) || odd(x, 15) || odd(w, 15) ||
+      odd(sx, 15) || odd(sw, 15) || odd(out, 15) || odd(residual, 15) || M > 0x7fffff00ll ||
+      (gate != 0 && (act != 0 || bias != nullptr || residual != nullptr)) ||
+      (tiles == nullptr ? groups != 1 : num_tiles == nullptr || bias != nullptr || residual != nullptr))
+    return -2;
+  const bool mx = fmt == kMxfp4;
+  static bool attr_set[64] = {false};
+  static int sm_count[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return -3;
+  if (!attr_set[dev]) {
+    if (cudaFuncSetAttribute(fp4_gemm_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
+            cudaSuccess ||
+        cudaFuncSetAttribute(fp4_gemm_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
+            cudaSuccess ||
+        cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return -3;
+    attr_set[dev] = true;
+  }
+  const int sms = sm_count[dev];
+  Fp4GemmArgs a;
+  memset(&a, 0, sizeof(a));
+  a.N = N;
+  a.M = (int)M;
+  a.kblocks = (K + kF4StepCols - 1) / kF4StepCols;
+  a.n_tiles = (N + 127) / 128;
+  a.bn = tiles != nullptr ? 128 : M <= 64 ? 64 : M <= 128 ? 128 : kF4MaxTokens;
+  a.m_tiles = (int)((M + a.bn - 1) / a.bn);
+  a.sfb_tiles = a.bn > 128 ? 2 : 1;
+  const int step_tiles = mx ? 2 : 4;
+  a.b_bytes = (uint32_t)a.bn * 128;
+  a.sfa_bytes = (uint32_t)step_tiles * kFp4ScaleTile;
+  a.sfb_bytes = a.sfa_bytes * (uint32_t)a.sfb_tiles;
+  a.w_row_tiles = a.n_tiles;
+  a.act = gate != 0 ? gate : act;
+  a.has_gate = gate != 0;
+  a.gate.limit = gate_limit;
+  a.gate.alpha = gate_alpha;
+  a.tiles = reinterpret_cast<const int4*>(tiles);
+  a.num_tiles = reinterpret_cast<const int*>(num_tiles);
+  a.x_scale = reinterpret_cast<const float*>(gx);
+  a.w_scale = reinterpret_cast<const float*>(gw);
+  a.bias = reinterpret_cast<const bf16*>(bias);
+  a.residual = reinterpret_cast<const bf16*>(residual);
+  a.ldr = ldr;
+  a.out = reinterpret_cast<bf16*>(out);
+  a.ldo = ldo;
+  a.status = status;
+  const uint64_t stage = kF4ABytes + a.b_bytes + a.sfa_bytes + a.sfb_bytes;
+  const uint64_t header = 256 + kF4EpilogueWarps * 32 * 4;
+  a.stages = (int)((227 * 1024 - header) / stage);
+  if (a.stages > kF4MaxStages) a.stages = kF4MaxStages;
+  const long long total = (long long)(tiles != nullptr ? max_tiles : a.m_tiles) * a.n_tiles;
+  if (total > 0x7fffffff) return -6;
+
+  const int k_tiles = fp4_k_tiles(K, mx);
+  const long long x_row_tiles = tiles != nullptr ? max_tiles : (M + 127) / 128;
+  CUtensorMap tw, tx, tsw, tsx;
+  {
+    const uint64_t dims[3] = {(uint64_t)K / 2, (uint64_t)N, (uint64_t)groups};
+    const uint64_t strides[2] = {(uint64_t)ldw, (uint64_t)(groups > 1 ? w_gstride : ldw)};
+    const uint32_t box[3] = {128, 128, 1};
+    if (make_tmap_nd(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, dims, strides, box) != 0) return -4;
+  }
+  if (make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K / 2, (uint64_t)ldx,
+                   (uint32_t)a.bn, 128) != 0)
+    return -4;
+  auto scales = [&](CUtensorMap* map, const void* base, uint64_t row_tiles, uint32_t box_tiles) {
+    const uint64_t dims[3] = {kFp4ScaleTile / 4, (uint64_t)k_tiles, row_tiles};
+    const uint64_t strides[2] = {kFp4ScaleTile, (uint64_t)k_tiles * kFp4ScaleTile};
+    const uint32_t box[3] = {kFp4ScaleTile / 4, (uint32_t)step_tiles, box_tiles};
+    return make_tmap_nd(map, base, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  if (scales(&tsw, sw, (uint64_t)groups * a.n_tiles, 1) != 0 ||
+      scales(&tsx, sx, (uint64_t)x_row_tiles, (uint32_t)a.sfb_tiles) != 0)
+    return -4;
+  const dim3 grid((unsigned)(total < sms ? total : sms));
+  const size_t smem = (size_t)(a.stages * stage + header);
+  const cudaError_t e = mx ? launch_pdl(fp4_gemm_kernel<true>, grid, dim3(kF4Threads), smem, stream, tw, tx, tsw, tsx, a)
+                           : launch_pdl(fp4_gemm_kernel<false>, grid, dim3(kF4Threads), smem, stream, tw, tx, tsw, tsx, a);
+  return e == cudaSuccess ? 0 : -5;
+}
+
+}  // extern "C"

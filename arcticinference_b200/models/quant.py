@@ -321,3 +321,187 @@ def linear_fp8_ref(x: torch.Tensor, w: Fp8Weight) -> torch.Tensor:
     M, K = x.shape
     xd = xq.float().view(M, K // BLOCK, BLOCK) * sx_t.t().unsqueeze(-1)
     return (xd.view(M, K) @ w.dequantize().float().t()).to(torch.bfloat16)
+
+
+# ------------------------------------------------------------------------ microscaled 4-bit numbers
+FP4_FORMATS = ("nvfp4", "mxfp4")
+FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+FP4_ROW_TILE, FP4_TILE_BYTES = 128, 512
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def check_fp4_format(fmt: str) -> str:
+    if fmt not in FP4_FORMATS:
+        raise ValueError("4-bit format %r: %s are there" % (fmt, " and ".join(FP4_FORMATS)))
+    return fmt
+
+
+def fp4_scale_tiles(rows: int, cols: int, fmt: str) -> tuple:
+    """Shape of the scale tiles of a [rows, cols] matrix."""
+    return (-(-rows // FP4_ROW_TILE), -(-cols // (4 * FP4_BLOCK[fmt])), FP4_TILE_BYTES)
+
+
+def tile_fp4_scales(s: torch.Tensor) -> torch.Tensor:
+    """Scale bytes [.., R, S] -> tiles [.., ceil(R / 128), ceil(S / 4), 512] (zeros beyond the matrix): byte
+    (r % 32) * 16 + (r // 32) * 4 + b of a tile is the scale of row r and block b, the order in which the tensor
+    core's scales are copied (csrc/common/fp4.cuh)."""
+    *lead, R, S = s.shape
+    p = torch.zeros(*lead, -(-R // FP4_ROW_TILE) * FP4_ROW_TILE, -(-S // 4) * 4, dtype=torch.uint8, device=s.device)
+    p[..., :R, :S] = s
+    n = len(lead)
+    p = p.reshape(*lead, p.shape[-2] // FP4_ROW_TILE, 4, 32, p.shape[-1] // 4, 4)
+    return p.permute(*range(n), n, n + 3, n + 2, n + 1, n + 4).reshape(*lead, -1, p.shape[-2], FP4_TILE_BYTES)
+
+
+def untile_fp4_scales(t: torch.Tensor, rows: int, blocks: int) -> torch.Tensor:
+    """The inverse: [.., row tiles, block tiles, 512] -> bytes [.., rows, blocks]."""
+    *lead, a, b, _ = t.shape
+    n = len(lead)
+    p = t.reshape(*lead, a, b, 32, 4, 4).permute(*range(n), n, n + 3, n + 2, n + 1, n + 4)
+    return p.reshape(*lead, a * FP4_ROW_TILE, b * 4)[..., :rows, :blocks]
+
+
+class Fp4Rows:
+    """A matrix of microscaled 4-bit numbers, quantised along its rows: the activations of a linear layer, or
+    (:class:`Fp4Weight`) its weight.
+
+    ``q`` uint8 [M, K / 2]: e2m1 codes, the even column in the low half of a byte. ``scale`` uint8: block scales in
+    tiles (:func:`tile_fp4_scales`). Formats: ``nvfp4``, blocks of 16 with an e4m3 scale and a factor per row, ``row_scale``
+    fp32 [M]; ``mxfp4``, blocks of 32 with an e8m0 scale (a power of two), ``row_scale`` None. With ``routing`` (rows
+    sorted by expert) row tile i of ``scale`` belongs to the router's i-th tile of rows."""
+
+    __slots__ = ("q", "scale", "row_scale", "fmt", "routing")
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, row_scale, fmt: str, routing=None):
+        check_fp4_format(fmt)
+        if q.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise ValueError("4-bit codes and scales are uint8 tensors")
+        if q.dim() not in (2, 3) or q.shape[-1] % 16:
+            raise ValueError("4-bit codes: [rows, K / 2] with K a multiple of 32, got %s" % (tuple(q.shape),))
+        tiles = fp4_scale_tiles(q.shape[-2], 2 * q.shape[-1], fmt)
+        if routing is not None:
+            tiles = (scale.shape[-3],) + tiles[1:]
+        if tuple(scale.shape) != tuple(q.shape[:-2]) + tiles:
+            raise ValueError("scale tiles %s do not belong to codes %s" % (tuple(scale.shape), tuple(q.shape)))
+        if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != q.shape[:-1]):
+            raise ValueError("row factors: fp32 %s" % (tuple(q.shape[:-1]),))
+        self.q = q
+        self.scale = scale
+        self.row_scale = row_scale
+        self.fmt = fmt
+        self.routing = routing
+
+    @property
+    def shape(self):
+        return torch.Size((*self.q.shape[:-1], 2 * self.q.shape[-1]))
+
+    @property
+    def device(self):
+        return self.q.device
+
+    @property
+    def is_cuda(self):
+        return self.q.is_cuda
+
+    def numel(self):
+        return 2 * self.q.numel()
+
+    def dequantize(self) -> torch.Tensor:
+        from .. import ops
+        return ops.dequant_fp4(self)
+
+
+class Fp4Weight(Fp4Rows):
+    """The weight [N, K] of a linear layer, or those of a layer's experts [E, N, K]. Behaves like the matrix as far as
+    model code needs: ``shape`` and slices of rows that start on a multiple of 128 (a scale tile)."""
+
+    __slots__ = ()
+
+    def __init__(self, q, scale, row_scale, fmt):
+        super().__init__(q, scale, row_scale, fmt)
+
+    def __getitem__(self, idx) -> "Fp4Weight":
+        rows = idx[0] if isinstance(idx, tuple) else idx
+        if self.q.dim() != 2 or not isinstance(rows, slice) or \
+                isinstance(idx, tuple) and (len(idx) != 2 or idx[1] != slice(None)):
+            raise ValueError("a 4-bit weight is sliced by rows")
+        a, b, step = rows.indices(self.q.shape[0])
+        if a % FP4_ROW_TILE or step != 1:
+            raise ValueError("slices of a 4-bit weight start on a multiple of %d rows" % FP4_ROW_TILE)
+        b = max(a, b)
+        return Fp4Weight(self.q[a:b], self.scale[a // FP4_ROW_TILE:-(-b // FP4_ROW_TILE)],
+                         None if self.row_scale is None else self.row_scale[a:b], self.fmt)
+
+    def requantize_from(self, dense: torch.Tensor) -> None:
+        """Overwrite codes and scales in place (addresses captured in CUDA graphs stay valid)."""
+        w = quantize_weight_fp4(dense, self.fmt)
+        self.q.copy_(w.q)
+        self.scale.copy_(w.scale)
+        if self.row_scale is not None:
+            self.row_scale.copy_(w.row_scale if w.row_scale is not None else torch.ones_like(self.row_scale))
+
+
+def quantize_fp4_ref(x: torch.Tensor, fmt: str) -> Fp4Rows:
+    """PyTorch restatement of ``csrc/quant_fp4.cu`` (formulas there): every step but the roundings to e4m3 and e2m1
+    is exact, so both give the same bits."""
+    size = FP4_BLOCK[check_fp4_format(fmt)]
+    b = x.double().reshape(*x.shape[:-1], x.shape[-1] // size, size)
+    top = b.abs().amax(-1)
+    if fmt == "mxfp4":
+        fine = torch.isfinite(top)
+        e = torch.frexp(torch.where(fine, top, 1.0)).exponent - 3
+        e = torch.where(fine & (top > 0), e, -127).clamp(min=-127)
+        scales = torch.where(fine, e + 127, 255).to(torch.uint8)
+        step, g = torch.where(fine, torch.ldexp(torch.ones_like(top), e), torch.inf), None
+    else:
+        most = top.amax(-1)
+        fine = torch.isfinite(most)
+        m, e = torch.frexp(torch.where(fine, most, 1.0) / 2688)
+        e = torch.where(m > 0.5, e, e - 1).clamp(min=-126)        # ceil(log2(..))
+        unit = torch.ldexp(torch.ones_like(most), torch.where(most > 0, e, 0))
+        s = torch.where(fine.unsqueeze(-1), top, 0.0) / unit.unsqueeze(-1) / 6
+        s = s.float().to(torch.float8_e4m3fn)
+        scales, step = s.view(torch.uint8), s.double() * unit.unsqueeze(-1)
+        g = torch.where(fine, unit, torch.nan).float()
+    a = torch.where((step > 0).unsqueeze(-1), b.abs() / step.unsqueeze(-1), 0.0)
+    a = torch.nan_to_num(a, nan=0.0)
+    code = (a > 0.25).to(torch.uint8)
+    for border, up in ((0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False)):
+        code += (a >= border) if up else (a > border)        # ties go to the even code
+    code = (code + 8 * (torch.signbit(b) & (step > 0).unsqueeze(-1) & torch.isfinite(b))).to(torch.uint8)
+    if fmt == "nvfp4":
+        code = torch.where(fine[..., None, None], code, 0)
+    else:
+        code = torch.where(fine.unsqueeze(-1), code, 0)
+    code = code.to(torch.uint8).reshape(*x.shape[:-1], x.shape[-1] // 2, 2)
+    return Fp4Rows(code[..., 0] | (code[..., 1] << 4), tile_fp4_scales(scales), g, fmt)
+
+
+def dequantize_fp4_ref(rows: Fp4Rows) -> torch.Tensor:
+    """The numbers that codes, scales and factors stand for, fp32."""
+    q = rows.q
+    nib = torch.stack([q & 15, q >> 4], -1).reshape(*q.shape[:-1], 2 * q.shape[-1]).long()
+    v = torch.tensor(E2M1 + tuple(-x for x in E2M1), dtype=torch.float32, device=q.device)[nib]
+    blocks = v.shape[-1] // FP4_BLOCK[rows.fmt]
+    s = untile_fp4_scales(rows.scale, q.shape[-2], blocks)
+    if rows.fmt == "nvfp4":
+        s = s.view(torch.float8_e4m3fn).float()
+    else:
+        s = torch.where(s == 255, torch.nan, torch.ldexp(torch.ones(s.shape, device=s.device), s.int() - 127))
+    v = (v.reshape(*s.shape, FP4_BLOCK[rows.fmt]) * s.unsqueeze(-1)).reshape(v.shape)
+    return v if rows.row_scale is None else v * rows.row_scale.unsqueeze(-1)
+
+
+def quantize_weight_fp4(w: torch.Tensor, fmt: str = "nvfp4") -> Fp4Weight:
+    """[N, K] or [E, N, K] -> 4-bit weight (values are taken as bf16)."""
+    from .. import ops
+    if w.dim() not in (2, 3) or w.shape[-1] % 32:
+        raise ValueError("4-bit quantisation needs [N, K] or [E, N, K] with K a multiple of 32, got %s" %
+                         (tuple(w.shape),))
+    w = w.to(torch.bfloat16)
+    parts = [ops.quant_fp4(m, fmt) for m in (w if w.dim() == 3 else w[None])]
+    if w.dim() == 2:
+        r = parts[0]
+        return Fp4Weight(r.q, r.scale, r.row_scale, fmt)
+    return Fp4Weight(torch.stack([r.q for r in parts]), torch.stack([r.scale for r in parts]),
+                     None if parts[0].row_scale is None else torch.stack([r.row_scale for r in parts]), fmt)

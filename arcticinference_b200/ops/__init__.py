@@ -22,6 +22,7 @@ __all__ = [
     "linear", "linear_fp8", "linear_fp8_row", "quant_fp8", "quant_fp8_row", "gemm_nn", "embedding", "rmsnorm", "layernorm", "silu_mul", "silu_mul_blocked", "rope_cache",
     "gather_rows", "argmax_sample", "AttentionMetadata", "build_attention_metadata", "pick_tile_keys", "plan_attention_work",
     "attention", "attention_masked", "attention_contiguous", "check_status", "count_launches", "launch_counter",
+    "quant_fp4", "dequant_fp4", "rmsnorm_fp4", "silu_mul_fp4", "linear_fp4", "grouped_linear_fp4",
 ]
 
 
@@ -382,11 +383,15 @@ def linear_fp8(x: torch.Tensor, w, out=None, force_splits: int = 0, peer=None,
 
 def linear(x: torch.Tensor, w, bias=None, residual=None, act=None, out=None,
            force_splits: int = 0, sync=None) -> torch.Tensor:
-    """``out = act(x @ w.T + bias) + residual``; x [M, K] (row stride free), w [N, K] bf16 or
-    an ``Fp8Weight``. ``sync``: optional ``native.PeerSync`` (wait for the ranks that produce
+    """``out = act(x @ w.T + bias) + residual``; x [M, K] (row stride free), w [N, K] bf16, an
+    ``Fp8Weight`` or an ``Fp4Weight``. ``sync``: optional ``native.PeerSync`` (wait for the ranks that produce
     ``x``, signal the ranks that consume ``out``)."""
     if not isinstance(w, torch.Tensor):
-        from ..models.quant import Fp8RowWeight
+        from ..models.quant import Fp4Weight, Fp8RowWeight
+        if isinstance(w, Fp4Weight):
+            if sync is not None:
+                raise ValueError("cross-rank ordering is not available for 4-bit linears")
+            return linear_fp4(x, w, bias, residual, act, out=out)
         if isinstance(w, Fp8RowWeight):
             return linear_fp8_row(x, w, bias, residual, act, out=out, force_splits=force_splits,
                                   sync=sync)
@@ -505,10 +510,12 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, vocab_start: int = 0, out=
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual=None, out=None,
-            quant: bool = False):
+            quant=False):
     """y = RMSNorm(x (+ residual)); ``residual`` (contiguous) is updated in place. With
     ``quant`` the result is a ``QuantAct`` (e4m3 rows with one scale per token, produced in the
-    same pass) for an fp8 linear layer."""
+    same pass) for an fp8 linear layer, with ``quant`` "nvfp4" or "mxfp4" ``Fp4Rows`` for a 4-bit one."""
+    if isinstance(quant, str):
+        return rmsnorm_fp4(x, weight, eps, residual, quant)
     if not x.is_cuda:
         y = ref.rmsnorm(x, weight, eps, residual)
         if quant:
@@ -561,9 +568,12 @@ def layernorm(x, gamma, beta, eps: float, residual=None):
     return out
 
 
-def silu_mul_blocked(x: torch.Tensor, nblk: int = 1, out=None, quant: bool = False):
+def silu_mul_blocked(x: torch.Tensor, nblk: int = 1, out=None, quant=False):
     """x: [T, nblk * 2 * I] as nblk blocks of (gate | up) -> [T, nblk * I]; with ``quant`` a
-    ``QuantAct`` of the same values (one scale per token over the whole output row)."""
+    ``QuantAct`` of the same values (one scale per token over the whole output row), with ``quant`` "nvfp4" or
+    "mxfp4" their ``Fp4Rows``."""
+    if isinstance(quant, str):
+        return silu_mul_fp4(x, nblk, quant)
     if not x.is_cuda:
         y = ref.silu_mul_blocked(x, nblk)
         if quant:
@@ -1305,3 +1315,7 @@ def attention_contiguous(q, k, v, seq_lens, H: int, D: int, scale: float | None 
     nat.check(rc, "attention_contiguous")
     launch_counter.add(1)
     return out
+
+
+from .fp4_ops import (dequant_fp4, grouped_linear_fp4, linear_fp4, quant_fp4, rmsnorm_fp4,  # noqa: E402
+                      silu_mul_fp4)

@@ -452,8 +452,12 @@ def _aligned(*ts) -> bool:
 
 
 def grouped_linear(x: torch.Tensor, w: torch.Tensor, routing: Routing, act=None):
-    """Rows sorted by expert [n, K] times each row's expert matrix of ``w`` [E, N, K]. With
-    ``act`` (a Gate) the matrices are interleaved gate / up ones, joined by it."""
+    """Rows sorted by expert [n, K] times each row's expert matrix of ``w`` [E, N, K] (bf16, or an
+    ``Fp4Weight``: both operands in 4 bits). With ``act`` (a Gate) the matrices are interleaved gate / up ones, joined
+    by it."""
+    if not isinstance(w, torch.Tensor):
+        from .fp4_ops import grouped_linear_fp4
+        return grouped_linear_fp4(x, w, routing, act)
     act = None if act is None else Gate.of(act)
     n, K = x.shape
     E, N, _ = w.shape
