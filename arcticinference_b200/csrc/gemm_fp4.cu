@@ -12,6 +12,7 @@
 // eight warps drain the other one. A lane then holds one feature of many tokens: four lanes exchange four by four
 // values and store eight bytes, 64 consecutive bytes per token and instruction.
 
+#include <stdlib.h>
 #include <string.h>
 
 #include "api.h"
@@ -29,9 +30,10 @@ constexpr int kF4Threads = (2 + kF4EpilogueWarps) * 32;
 constexpr int kF4MaxStages = 10;
 constexpr int kF4StepCols = 256;                       // columns of a stage: 128 bytes of codes
 constexpr uint32_t kF4ABytes = 128 * 128;
-constexpr uint32_t kF4ScaleAt = 384;                   // tensor memory: accumulators at 0 and 192, then two sets of scales
-constexpr uint32_t kF4ScaleSet = 64;
-constexpr int kF4MaxTokens = 192;
+// Tensor memory: columns 0 - 383 for two accumulators, then two sets of scales. An accumulator of more than 128 tokens
+// takes columns 0 - 255 or 128 - 383: the middle ones belong to both, are drained first and handed on at once.
+constexpr uint32_t kF4Middle = 128, kF4ScaleAt = 384, kF4ScaleSet = 64;
+constexpr int kF4MaxTokens = 256;
 
 struct Fp4GemmArgs {
   int N, M, kblocks, n_tiles, m_tiles;
@@ -61,7 +63,6 @@ struct F4Work {
   int shift;               // first token's place in it, in columns of 32
 };
 
-template <bool PAIR>
 __device__ __forceinline__ F4Work f4_work(const Fp4GemmArgs& p, int w) {
   F4Work r;
   if (p.tiles != nullptr) {
@@ -90,6 +91,11 @@ __device__ __forceinline__ F4Work f4_work(const Fp4GemmArgs& p, int w) {
 
 // Columns of the instruction: what a tile has, in steps of 16
 __device__ __forceinline__ int f4_width(int nrows) { return (nrows + 15) & ~15; }
+
+// First column of an accumulator: side columns 0 - 127 or 256 - 383 with the middle ones between them
+__device__ __forceinline__ uint32_t f4_accumulator(int acc, int nrows) {
+  return acc == 0 ? 0u : nrows > (int)kF4Middle ? kF4Middle : 2u * kF4Middle;
+}
 
 __device__ __forceinline__ float gelu_exact(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752f)); }
 
@@ -169,7 +175,7 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
   }
 }
 
-template <bool MX>
+template <bool MX, bool PAIR>
 __global__ void __launch_bounds__(kF4Threads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                 const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
@@ -182,9 +188,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (threadIdx.x == 0) report_error(p.status, kErrBadArgument, 1500, (int)(smem_u32(smem) & 1023u));
     return;
   }
+  constexpr int kTiles = MX ? 2 : 4;      // scale tiles of a step
+  constexpr int kCtas = PAIR ? 2 : 1;
   const uint32_t stage_bytes = kF4ABytes + p.b_bytes + p.sfa_bytes + p.sfb_bytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * stage_bytes);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kF4MaxStages + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kF4MaxStages + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* cols = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);   // 32 floats a warp
   const uint32_t smem_base = smem_u32(smem);
@@ -192,9 +200,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   auto full_bar = [&](int s) { return bars_base + 8u * s; };
   auto empty_bar = [&](int s) { return bars_base + 8u * (kF4MaxStages + s); };
   auto tfull_bar = [&](int a) { return bars_base + 8u * (2 * kF4MaxStages + a); };
-  auto tempty_bar = [&](int a) { return bars_base + 8u * (2 * kF4MaxStages + 2 + a); };
+  auto side_bar = [&](int a) { return bars_base + 8u * (2 * kF4MaxStages + 2 + a); };
+  const uint32_t middle_bar = bars_base + 8u * (2 * kF4MaxStages + 4);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -203,8 +213,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), kF4EpilogueWarps);
+      mbar_init(side_bar(a), kCtas * kF4EpilogueWarps);   // (the even CTA's: both CTAs drain)
     }
+    mbar_init(middle_bar, kCtas * kF4EpilogueWarps);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tensormap(&tmap_w);
@@ -213,16 +224,23 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     prefetch_tensormap(&tmap_sx);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();   // the other CTA's barriers are ready for this one's copies and arrivals
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();   // (tensor memory is owned)
   pdl_wait();
   const int total_work = (p.tiles != nullptr ? *p.num_tiles : p.m_tiles) * p.n_tiles;
+  const int first_work = (int)blockIdx.x / kCtas, work_step = (int)gridDim.x / kCtas;
 
   if (warp == 0) {
     // ------------------------------ TMA producer ------------------------------
@@ -230,30 +248,39 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int w = blockIdx.x; w < total_work && ok; w += gridDim.x) {
-        const F4Work t = f4_work<false>(p, w);
+      for (int w = first_work; w < total_work && ok; w += work_step) {
+        const F4Work t = f4_work(p, w);
         if (t.nrows <= 0) continue;
-        const int feature0 = t.nt * 128;
+        const int slice = kCtas * t.nt + rank;       // 128 features
+        const int row = t.row0 + rank * (f4_width(t.nrows) / 2);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 1500 + stage, kb)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
+          // (pairs: one barrier, the even CTA's, collects the copies of both)
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), kCtas * stage_bytes);
+          const uint32_t full = PAIR ? map_to_cta(full_bar(stage), 0) : full_bar(stage);
           const uint32_t dst = smem_base + (uint32_t)stage * stage_bytes;
           const uint32_t sfa = dst + kF4ABytes + p.b_bytes;
-          constexpr int kTiles = MX ? 2 : 4;
-          tma_load_3d(dst, &tmap_w, full_bar(stage), kb * 128, feature0, t.group);
-          tma_load_2d(dst + kF4ABytes, &tmap_x, full_bar(stage), kb * 128, t.row0);
-          tma_load_3d(sfa, &tmap_sw, full_bar(stage), 0, kb * kTiles, t.group * p.w_row_tiles + t.nt);
-          tma_load_3d(sfa + p.sfa_bytes, &tmap_sx, full_bar(stage), 0, kb * kTiles, t.slot);
+          if (PAIR) {
+            tma_load_3d_pair(dst, &tmap_w, full, kb * 128, slice * 128, t.group);
+            tma_load_2d_pair(dst + kF4ABytes, &tmap_x, full, kb * 128, row);
+            tma_load_3d_pair(sfa, &tmap_sw, full, 0, kb * kTiles, t.group * p.w_row_tiles + slice);
+            tma_load_3d_pair(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, t.slot);
+          } else {
+            tma_load_3d(dst, &tmap_w, full, kb * 128, slice * 128, t.group);
+            tma_load_2d(dst + kF4ABytes, &tmap_x, full, kb * 128, row);
+            tma_load_3d(sfa, &tmap_sw, full, 0, kb * kTiles, t.group * p.w_row_tiles + slice);
+            tma_load_3d(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, t.slot);
+          }
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      if (!ok) {   // copies already issued get a short time to land
+      if (!ok) {   // copies already issued, by either CTA, get a short time to land
         const unsigned long long t0 = globaltimer_ns();
         while (globaltimer_ns() - t0 < 20000000ull) {
         }
@@ -262,108 +289,141 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   } else if (warp == 1) {
     // ------------------------------- MMA issuer -------------------------------
     // (uniform control and one elected lane, see gemm_bf16.cu)
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
-    const uint64_t a0 = make_desc_kmajor_sw128(smem_base);
-    const uint64_t s0 = make_desc_scales(smem_base + kF4ABytes + p.b_bytes);
-    const uint64_t stage_step = stage_bytes / 16;
-    const uint32_t sfb_cols = 4u * (uint32_t)p.sfb_tiles;
-    constexpr int kTiles = MX ? 2 : 4;
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    // the stages of the last step and of the one before: its products must be done before its set of scales is
-    // written again
-    int last_stage = -1, old_stage = -1;
-    uint32_t last_phase = 0, old_phase = 0, set = 0;
-    bool ok = true;
-    for (int w = blockIdx.x; w < total_work && ok; w += gridDim.x) {
-      const F4Work t = f4_work<false>(p, w);
-      if (t.nrows <= 0) continue;
-      if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.status,
-                                             1600 + acc, w)))
-        break;
-      tc_fence_after();
-      const uint32_t n = (uint32_t)f4_width(t.nrows);
-      const uint32_t idesc = make_idesc_fp4(128, n, MX, 0), idesc_hi = make_idesc_fp4(128, n, MX, 2);
-      const uint32_t d_tmem = tm + (uint32_t)acc * (uint32_t)kF4MaxTokens;
-      for (int kb = 0; kb < p.kblocks; ++kb) {
-        if (old_stage >= 0 && !__all_sync(0xffffffffu, mbar_wait(empty_bar(old_stage), old_phase, abort_flag,
-                                                                 p.status, 1620 + stage, kb))) {
-          ok = false;
+    if (rank == 0) {
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint64_t a0 = make_desc_kmajor_sw128(smem_base);
+      const uint64_t s0 = make_desc_scales(smem_base + kF4ABytes + p.b_bytes);
+      const uint64_t stage_step = stage_bytes / 16;
+      const uint32_t sfb_cols = 4u * (uint32_t)p.sfb_tiles;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, side_phase = 0, middle_phase = 0;
+      // the stages of the last step and of the one before: its products must be done before its set of scales is
+      // written again
+      int last_stage = -1, old_stage = -1;
+      uint32_t last_phase = 0, old_phase = 0, set = 0;
+      bool ok = true;
+      for (int w = first_work; w < total_work && ok; w += work_step) {
+        const F4Work t = f4_work(p, w);
+        if (t.nrows <= 0) continue;
+        if (!__all_sync(0xffffffffu, mbar_wait(side_bar(acc), side_phase ^ 1u, abort_flag, p.status, 1600 + acc, w)))
           break;
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.status, 1640 + stage, kb))) {
-          ok = false;
-          break;
+        if (t.nrows > (int)kF4Middle) {
+          if (!__all_sync(0xffffffffu, mbar_wait(middle_bar, middle_phase ^ 1u, abort_flag, p.status, 1610, w))) break;
+          middle_phase ^= 1u;
         }
         tc_fence_after();
-        const uint64_t a_desc = a0 + (uint64_t)stage * stage_step;
-        const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
-        const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
-        const uint64_t sb_desc = sa_desc + (uint64_t)(p.sfa_bytes / 16);
-        const uint32_t sfa = tm + kF4ScaleAt + set * kF4ScaleSet, sfb = sfa + 16u;
-        if (elect_one()) {
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            tmem_copy_scales<false>(sfa + 4u * j, sa_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
-            for (int i = 0; i < p.sfb_tiles; ++i)
-              tmem_copy_scales<false>(sfb + sfb_cols * j + 4u * i,
-                                      sb_desc + (uint64_t)((i * kTiles + j) * (kFp4ScaleTile / 16)));
+        const uint32_t n = (uint32_t)f4_width(t.nrows);
+        const uint32_t idesc = make_idesc_fp4(128 * kCtas, n, MX, 0), idesc_hi = make_idesc_fp4(128 * kCtas, n, MX, 2);
+        const uint32_t d_tmem = tm + f4_accumulator(acc, t.nrows);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (old_stage >= 0 && !__all_sync(0xffffffffu, mbar_wait(empty_bar(old_stage), old_phase, abort_flag,
+                                                                   p.status, 1620 + stage, kb))) {
+            ok = false;
+            break;
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int j = MX ? k / 2 : k;
-            umma_fp4_ss<MX, false>(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
-                                   MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j,
-                                   sfb + sfb_cols * j + (uint32_t)t.shift, (kb > 0 || k > 0) ? 1u : 0u);
+          if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.status, 1640 + stage, kb))) {
+            ok = false;
+            break;
           }
-          tc_commit(empty_bar(stage));
-          if (kb == p.kblocks - 1) tc_commit(tfull_bar(acc));
+          tc_fence_after();
+          const uint64_t a_desc = a0 + (uint64_t)stage * stage_step;
+          const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
+          const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
+          const uint64_t sb_desc = sa_desc + (uint64_t)(p.sfa_bytes / 16);
+          const uint32_t sfa = tm + kF4ScaleAt + set * kF4ScaleSet, sfb = sfa + 16u;
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              tmem_copy_scales<PAIR>(sfa + 4u * j, sa_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
+              for (int i = 0; i < p.sfb_tiles; ++i)
+                tmem_copy_scales<PAIR>(sfb + sfb_cols * j + 4u * i,
+                                       sb_desc + (uint64_t)((i * kTiles + j) * (kFp4ScaleTile / 16)));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int j = MX ? k / 2 : k;
+              umma_fp4_ss<MX, PAIR>(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
+                                    MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j,
+                                    sfb + sfb_cols * j + (uint32_t)t.shift, (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            if (PAIR) {
+              tc_commit_pair(empty_bar(stage));
+              if (kb == p.kblocks - 1) tc_commit_pair(tfull_bar(acc));
+            } else {
+              tc_commit(empty_bar(stage));
+              if (kb == p.kblocks - 1) tc_commit(tfull_bar(acc));
+            }
+          }
+          __syncwarp();
+          old_stage = last_stage;
+          old_phase = last_phase;
+          last_stage = stage;
+          last_phase = phase;
+          set ^= 1u;
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
-        __syncwarp();
-        old_stage = last_stage;
-        old_phase = last_phase;
-        last_stage = stage;
-        last_phase = phase;
-        set ^= 1u;
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (!ok) break;
+        acc ^= 1;
+        if (acc == 0) side_phase ^= 1u;
       }
-      if (!ok) break;
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
     }
   } else {
     // --------------------------------- epilogue --------------------------------
     const int quad = warp & 3;            // TMEM lane quadrant this warp may read
     const int half = (warp - 2) >> 2;     // which of the quadrant's two warps this is
     float* my_cols = cols + (warp - 2) * 32;
+    auto hand_back = [&](uint32_t bar) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(map_to_cta(bar, 0));
+        else mbar_arrive(bar);
+      }
+    };
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int w = blockIdx.x; w < total_work; w += gridDim.x) {
-      const F4Work t = f4_work<false>(p, w);
+    for (int w = first_work; w < total_work; w += work_step) {
+      const F4Work t = f4_work(p, w);
       if (t.nrows <= 0) continue;
-      const int feature0 = t.nt * 128 + quad * 32;
+      const int feature0 = (kCtas * t.nt + rank) * 128 + quad * 32;
       const int f = min(feature0 + lane, p.N - 1);
       const float h = p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f;
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 1700 + acc, w)))
         break;
       tc_fence_after();
-      const uint32_t t_addr = tmem_base + (uint32_t)acc * (uint32_t)kF4MaxTokens + ((uint32_t)(quad * 32) << 16);
-      for (int c0 = 32 * half; c0 < t.nrows && feature0 < p.N; c0 += 64) {
-        uint32_t r[32];
+      const uint32_t t_addr = tmem_base + f4_accumulator(acc, t.nrows) + ((uint32_t)(quad * 32) << 16);
+      // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and both
+      // handed back as soon as they are in registers.
+      const bool wide = t.nrows > (int)kF4Middle;
+      const int first = wide && acc == 0 ? 128 : 0;
+      for (int part = 0; part < (wide ? 2 : 1); ++part) {
+        const int c0 = (part == 0 ? first : 128 - first) + 32 * half;
+        const bool any0 = c0 < t.nrows && feature0 < p.N, any1 = c0 + 64 < t.nrows && feature0 < p.N;
+        uint32_t r0[32], r1[32];
         __syncwarp();
-        tmem_ld_x32(t_addr + (uint32_t)c0, r);
-        my_cols[lane] = p.x_scale != nullptr && c0 + lane < t.nrows ? p.x_scale[t.row0 + c0 + lane] : 1.f;
-        __syncwarp();
-        tmem_ld_wait_dep(r);
-        f4_store32(p, r, my_cols, c0, t.row0, t.nrows, feature0, h, bias, lane);
+        if (any0) tmem_ld_x32(t_addr + (uint32_t)c0, r0);
+        if (any1) tmem_ld_x32(t_addr + (uint32_t)(c0 + 64), r1);
+        if (any0) tmem_ld_wait_dep(r0);
+        if (any1) tmem_ld_wait_dep(r1);
+        hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
+        auto factors = [&](int c) {
+          __syncwarp();
+          my_cols[lane] = p.x_scale != nullptr && c + lane < t.nrows ? p.x_scale[t.row0 + c + lane] : 1.f;
+          __syncwarp();
+        };
+        if (any0) {
+          factors(c0);
+          f4_store32(p, r0, my_cols, c0, t.row0, t.nrows, feature0, h, bias, lane);
+        }
+        if (any1) {
+          factors(c0 + 64);
+          f4_store32(p, r1, my_cols, c0 + 64, t.row0, t.nrows, feature0, h, bias, lane);
+        }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tempty_bar(acc));
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
@@ -371,9 +431,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();   // neither CTA leaves while the other may still signal it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if (PAIR) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -409,10 +471,11 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return -3;
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(fp4_gemm_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(fp4_gemm_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
-            cudaSuccess ||
+    auto large = [](auto kernel) {
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess;
+    };
+    if (large(fp4_gemm_kernel<false, false>) || large(fp4_gemm_kernel<true, false>) ||
+        large(fp4_gemm_kernel<false, true>) || large(fp4_gemm_kernel<true, true>) ||
         cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return -3;
     attr_set[dev] = true;
@@ -423,15 +486,19 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   a.N = N;
   a.M = (int)M;
   a.kblocks = (K + kF4StepCols - 1) / kF4StepCols;
-  a.n_tiles = (N + 127) / 128;
-  a.bn = tiles != nullptr ? 128 : M <= 64 ? 64 : M <= 128 ? 128 : kF4MaxTokens;
+  const char* forced = getenv("F4_PAIR");
+  const bool pair = forced != nullptr ? forced[0] == '1' : tiles != nullptr ? max_tiles > 4 * groups : M > 128;
+  a.n_tiles = (N + (pair ? 255 : 127)) / (pair ? 256 : 128);
+  const long long split = (M + kF4MaxTokens - 1) / kF4MaxTokens;      // tiles of equal width, in steps of 64
+  a.bn = tiles != nullptr ? 128 : (int)(((M + split - 1) / split + 63) / 64 * 64);
+  if (getenv("F4_BN") && M > 256) a.bn = atoi(getenv("F4_BN"));
   a.m_tiles = (int)((M + a.bn - 1) / a.bn);
   a.sfb_tiles = a.bn > 128 ? 2 : 1;
   const int step_tiles = mx ? 2 : 4;
-  a.b_bytes = (uint32_t)a.bn * 128;
+  a.b_bytes = (uint32_t)(pair ? a.bn / 2 : a.bn) * 128;
   a.sfa_bytes = (uint32_t)step_tiles * kFp4ScaleTile;
   a.sfb_bytes = a.sfa_bytes * (uint32_t)a.sfb_tiles;
-  a.w_row_tiles = a.n_tiles;
+  a.w_row_tiles = (N + 127) / 128;
   a.act = gate != 0 ? gate : act;
   a.has_gate = gate != 0;
   a.gate.limit = gate_limit;
@@ -463,7 +530,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
     if (make_tmap_nd(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, dims, strides, box) != 0) return -4;
   }
   if (make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K / 2, (uint64_t)ldx,
-                   (uint32_t)a.bn, 128) != 0)
+                   (uint32_t)(pair ? a.bn / 2 : a.bn), 128) != 0)
     return -4;
   auto scales = [&](CUtensorMap* map, const void* base, uint64_t row_tiles, uint32_t box_tiles) {
     const uint64_t dims[3] = {kFp4ScaleTile / 4, (uint64_t)k_tiles, row_tiles};
@@ -471,13 +538,17 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
     const uint32_t box[3] = {kFp4ScaleTile / 4, (uint32_t)step_tiles, box_tiles};
     return make_tmap_nd(map, base, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
   };
-  if (scales(&tsw, sw, (uint64_t)groups * a.n_tiles, 1) != 0 ||
+  if (scales(&tsw, sw, (uint64_t)groups * a.w_row_tiles, 1) != 0 ||
       scales(&tsx, sx, (uint64_t)x_row_tiles, (uint32_t)a.sfb_tiles) != 0)
     return -4;
-  const dim3 grid((unsigned)(total < sms ? total : sms));
   const size_t smem = (size_t)(a.stages * stage + header);
-  const cudaError_t e = mx ? launch_pdl(fp4_gemm_kernel<true>, grid, dim3(kF4Threads), smem, stream, tw, tx, tsw, tsx, a)
-                           : launch_pdl(fp4_gemm_kernel<false>, grid, dim3(kF4Threads), smem, stream, tw, tx, tsw, tsx, a);
+  const long long most = pair ? sms / 2 : sms;
+  const dim3 grid((unsigned)((total < most ? total : most) * (pair ? 2 : 1)));
+  auto go = [&](auto kernel) {
+    return launch_pdl_cluster(kernel, grid, dim3(kF4Threads), smem, stream, pair ? 2u : 1u, tw, tx, tsw, tsx, a);
+  };
+  const cudaError_t e = mx ? (pair ? go(fp4_gemm_kernel<true, true>) : go(fp4_gemm_kernel<true, false>))
+                           : (pair ? go(fp4_gemm_kernel<false, true>) : go(fp4_gemm_kernel<false, false>));
   return e == cudaSuccess ? 0 : -5;
 }
 
