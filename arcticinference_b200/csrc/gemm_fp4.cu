@@ -9,8 +9,7 @@
 // there are tokens, so a single token or a ragged group costs what it has. One thread feeds a ring of stages by TMA:
 // 256 columns of both operands (128 bytes a row, 128-byte swizzle) and their scale tiles. One warp copies a stage's
 // scales to tensor memory (two sets, used in turn) and issues the products into one of two accumulators;
-// eight warps drain the other one. A lane then holds one feature of many tokens: four lanes exchange four by four
-// values and store eight bytes, 64 consecutive bytes per token and instruction.
+// eight warps drain the other one.
 
 #include <stdlib.h>
 #include <string.h>
@@ -28,6 +27,7 @@ typedef __nv_bfloat16 bf16;
 constexpr int kF4EpilogueWarps = 8;
 constexpr int kF4Threads = (2 + kF4EpilogueWarps) * 32;
 constexpr int kF4MaxStages = 10;
+constexpr int kF4StoreBytes = 32 * 64;                 // a warp's staging tile
 constexpr int kF4StepCols = 256;                       // columns of a stage: 128 bytes of codes
 constexpr uint32_t kF4ABytes = 128 * 128;
 // Tensor memory: columns 0 - 383 for two accumulators, then two sets of scales. An accumulator of more than 128 tokens
@@ -111,71 +111,112 @@ __device__ __forceinline__ float f4_gated(int act, const GateParams& p, float g,
   return __fdividef(g, 1.f + __expf(-t)) * u;
 }
 
-// v[i]: token i's value of this lane's feature; afterwards lane 4 a + q has token q's features 4 a .. 4 a + 3.
-__device__ __forceinline__ void f4_transpose4(float (&v)[4], int lane) {
-  const bool odd = lane & 1, high = lane & 2;
-  float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
-  float s1 = __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
-  const float a0 = odd ? s0 : v[0], a1 = odd ? v[1] : s0;     // token 0 or 1: features f, f + 1
-  const float b0 = odd ? s1 : v[2], b1 = odd ? v[3] : s1;     // token 2 or 3
-  s0 = __shfl_xor_sync(0xffffffffu, high ? a0 : b0, 2);
-  s1 = __shfl_xor_sync(0xffffffffu, high ? a1 : b1, 2);
-  v[0] = high ? s0 : a0;
-  v[1] = high ? s1 : a1;
-  v[2] = high ? b0 : s0;
-  v[3] = high ? b1 : s1;
+// The factors and biases of a lane's four features of a warp's 32: l / 4 and every eighth after it.
+struct F4Features {
+  float h[4], bias[4];
+};
+
+// A warp's staging tile: [32 tokens][32 features] bf16, the 16-byte pieces of a token's 64 bytes permuted so that eight
+// tokens' equal pieces (a matrix fragment) lie in different banks
+__device__ __forceinline__ uint32_t f4_piece(int token, int piece) {
+  return (uint32_t)(token * 64 + ((piece ^ (token >> 1)) & 3) * 16);
 }
 
-// 32 tokens from c0 on of a finished tile; the lane's feature is feature0 + lane. cols: the tokens' factors.
-__device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t (&r)[32], const float* cols, int c0,
-                                           int row0, int nrows, int feature0, float h, float bias, int lane) {
+// Tokens c0 .. c0 + 31 of a finished tile: lo, hi the warp's first and last 16 features (tmem_ld_frag_x4). Fragments
+// are transposed through the staging tile, so that a store has 64 consecutive bytes of eight tokens. Moving them by
+// shuffles, four by four, cost three times the shared-memory cycles, which the products are short of.
+__device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t (&lo)[16], const uint32_t (&hi)[16],
+                                           uint8_t* stage, int c0, int row0, int nrows, int feature0,
+                                           const F4Features& ft, int lane) {
+  const uint32_t at = smem_u32(stage);
+  float2 g[4];
+  __syncwarp();   // (the tile's last readers are done)
+  if (p.x_scale != nullptr) {
+    float* cols = reinterpret_cast<float*>(stage);
+    cols[lane] = c0 + lane < nrows ? p.x_scale[row0 + c0 + lane] : 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = *reinterpret_cast<const float2*>(cols + 8 * j + 2 * (lane & 3));
+    __syncwarp();
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = make_float2(1.f, 1.f);
+  }
+  const uint32_t frag = at + f4_piece(lane & 7, lane >> 3);   // + 512 per eight tokens
   if (p.has_gate) {
-    // lanes 0 - 15: gate rows, 16 - 31 their up rows. The lower half joins the even tokens, the upper the odd ones.
-    const int f = (feature0 >> 1) + (lane & 12);
-    const bool up = lane >= 16;
+    // 16 gate rows, then the 16 up rows they belong to
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float v[4];
+    for (int j = 0; j < 4; ++j) {
+      uint32_t q[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 8 * i + 2 * j;
-        const float2 g = *reinterpret_cast<const float2*>(cols + t);
-        const float even = __uint_as_float(r[t]) * (g.x * h), odd = __uint_as_float(r[t + 1]) * (g.y * h);
-        const float other = __shfl_xor_sync(0xffffffffu, up ? even : odd, 16);
-        v[j] = f4_gated(p.act, p.gate, up ? other : even, up ? odd : other);
+      for (int i = 0; i < 2; ++i) {
+        const float a = f4_gated(p.act, p.gate, __uint_as_float(lo[4 * j + 2 * i]) * (g[j].x * ft.h[i]),
+                                 __uint_as_float(hi[4 * j + 2 * i]) * (g[j].x * ft.h[2 + i]));
+        const float b = f4_gated(p.act, p.gate, __uint_as_float(lo[4 * j + 2 * i + 1]) * (g[j].y * ft.h[i]),
+                                 __uint_as_float(hi[4 * j + 2 * i + 1]) * (g[j].y * ft.h[2 + i]));
+        q[i] = pack_bf16x2(a, b);
       }
-      f4_transpose4(v, lane);
-      const int t = c0 + 8 * i + 2 * (lane & 3) + (up ? 1 : 0);
-      if (t < nrows && 2 * f < p.N)
-        store4(p.out + (long long)(row0 + t) * p.ldo + f, make_float4(v[0], v[1], v[2], v[3]));
+      stmatrix_t2(frag + 512u * j, q[0], q[1]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = 16 * i + (lane >> 1), f = (feature0 >> 1) + 8 * (lane & 1);
+      if (c0 + t < nrows)
+        *reinterpret_cast<uint4*>(p.out + (long long)(row0 + c0 + t) * p.ldo + f) =
+            *reinterpret_cast<const uint4*>(stage + f4_piece(t, lane & 1));
     }
     return;
   }
-  const int f = feature0 + (lane & ~3);
+  const int f = feature0 + 8 * (lane & 3);
+  if (p.residual != nullptr) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (c0 + 4 * i >= nrows) break;
-    const float4 g = *reinterpret_cast<const float4*>(cols + 4 * i);
-    float v[4] = {__uint_as_float(r[4 * i]) * (g.x * h) + bias, __uint_as_float(r[4 * i + 1]) * (g.y * h) + bias,
-                  __uint_as_float(r[4 * i + 2]) * (g.z * h) + bias, __uint_as_float(r[4 * i + 3]) * (g.w * h) + bias};
+    for (int i = 0; i < 4; ++i) {
+      const int t = 8 * i + (lane >> 2);
+      if (c0 + t < nrows && f < p.N)
+        *reinterpret_cast<uint4*>(stage + f4_piece(t, lane & 3)) =
+            *reinterpret_cast<const uint4*>(p.residual + (long long)(row0 + c0 + t) * p.ldr + f);
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (c0 + 8 * j >= nrows) break;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t* r = (i < 2 ? lo : hi) + 4 * j + 2 * (i & 1);
+      v[2 * i] = __uint_as_float(r[0]) * (g[j].x * ft.h[i]) + ft.bias[i];
+      v[2 * i + 1] = __uint_as_float(r[1]) * (g[j].y * ft.h[i]) + ft.bias[i];
+    }
     if (p.act == 1) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = gelu_exact(v[j]);
+      for (int i = 0; i < 8; ++i) v[i] = gelu_exact(v[i]);
     }
-    f4_transpose4(v, lane);
-    const int t = c0 + 4 * i + (lane & 3);
-    if (t < nrows && f < p.N) {
-      const long long row = row0 + t;
-      if (p.residual != nullptr) {
-        const float4 a = load4(p.residual + row * p.ldr + f);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    if (p.residual != nullptr) {
+      uint32_t r[4];
+      ldmatrix_t4(frag + 512u * j, r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r[i]));
+        v[2 * i] += a.x;
+        v[2 * i + 1] += a.y;
       }
-      store4(p.out + row * p.ldo + f, make_float4(v[0], v[1], v[2], v[3]));
     }
+    stmatrix_t4(frag + 512u * j, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                pack_bf16x2(v[6], v[7]));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 8 * i + (lane >> 2);
+    if (c0 + t < nrows && f < p.N)
+      *reinterpret_cast<uint4*>(p.out + (long long)(row0 + c0 + t) * p.ldo + f) =
+          *reinterpret_cast<const uint4*>(stage + f4_piece(t, lane & 3));
   }
 }
 
-template <bool MX, bool PAIR>
+template <bool MX, bool PAIR, int SFB>
 __global__ void __launch_bounds__(kF4Threads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                 const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
@@ -194,7 +235,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * stage_bytes);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kF4MaxStages + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* cols = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);   // 32 floats a warp
+  uint8_t* store_stage = reinterpret_cast<uint8_t*>(bars) + 256;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bars_base = smem_u32(bars);
   auto full_bar = [&](int s) { return bars_base + 8u * s; };
@@ -294,7 +335,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       const uint64_t a0 = make_desc_kmajor_sw128(smem_base);
       const uint64_t s0 = make_desc_scales(smem_base + kF4ABytes + p.b_bytes);
       const uint64_t stage_step = stage_bytes / 16;
-      const uint32_t sfb_cols = 4u * (uint32_t)p.sfb_tiles;
+      constexpr uint32_t kSfaBytes = kTiles * kFp4ScaleTile;
       int stage = 0, acc = 0;
       uint32_t phase = 0, side_phase = 0, middle_phase = 0;
       // the stages of the last step and of the one before: its products must be done before its set of scales is
@@ -312,9 +353,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           middle_phase ^= 1u;
         }
         tc_fence_after();
-        const uint32_t n = (uint32_t)f4_width(t.nrows);
+        // (from the list: the same in all lanes, which the compiler cannot know)
+        const uint32_t n = __shfl_sync(0xffffffffu, (uint32_t)f4_width(t.nrows), 0);
+        const uint32_t shift = __shfl_sync(0xffffffffu, (uint32_t)t.shift, 0);
         const uint32_t idesc = make_idesc_fp4(128 * kCtas, n, MX, 0), idesc_hi = make_idesc_fp4(128 * kCtas, n, MX, 2);
-        const uint32_t d_tmem = tm + f4_accumulator(acc, t.nrows);
+        const uint32_t d_tmem = __shfl_sync(0xffffffffu, tm + f4_accumulator(acc, t.nrows), 0);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (old_stage >= 0 && !__all_sync(0xffffffffu, mbar_wait(empty_bar(old_stage), old_phase, abort_flag,
                                                                    p.status, 1620 + stage, kb))) {
@@ -329,14 +372,16 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           const uint64_t a_desc = a0 + (uint64_t)stage * stage_step;
           const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
           const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
-          const uint64_t sb_desc = sa_desc + (uint64_t)(p.sfa_bytes / 16);
+          const uint64_t sb_desc = sa_desc + (uint64_t)(kSfaBytes / 16);
           const uint32_t sfa = tm + kF4ScaleAt + set * kF4ScaleSet, sfb = sfa + 16u;
+          const uint32_t sfb_first = sfb + shift;
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < kTiles; ++j) {
               tmem_copy_scales<PAIR>(sfa + 4u * j, sa_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
-              for (int i = 0; i < p.sfb_tiles; ++i)
-                tmem_copy_scales<PAIR>(sfb + sfb_cols * j + 4u * i,
+#pragma unroll
+              for (int i = 0; i < SFB; ++i)
+                tmem_copy_scales<PAIR>(sfb + 4u * (SFB * j + i),
                                        sb_desc + (uint64_t)((i * kTiles + j) * (kFp4ScaleTile / 16)));
             }
 #pragma unroll
@@ -344,7 +389,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
               const int j = MX ? k / 2 : k;
               umma_fp4_ss<MX, PAIR>(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
                                     MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j,
-                                    sfb + sfb_cols * j + (uint32_t)t.shift, (kb > 0 || k > 0) ? 1u : 0u);
+                                    sfb_first + 4u * SFB * j, (kb > 0 || k > 0) ? 1u : 0u);
             }
             if (PAIR) {
               tc_commit_pair(empty_bar(stage));
@@ -374,7 +419,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     // --------------------------------- epilogue --------------------------------
     const int quad = warp & 3;            // TMEM lane quadrant this warp may read
     const int half = (warp - 2) >> 2;     // which of the quadrant's two warps this is
-    float* my_cols = cols + (warp - 2) * 32;
+    uint8_t* my_stage = store_stage + (warp - 2) * kF4StoreBytes;
     auto hand_back = [&](uint32_t bar) {
       tc_fence_before();
       __syncwarp();
@@ -389,9 +434,13 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       const F4Work t = f4_work(p, w);
       if (t.nrows <= 0) continue;
       const int feature0 = (kCtas * t.nt + rank) * 128 + quad * 32;
-      const int f = min(feature0 + lane, p.N - 1);
-      const float h = p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f;
-      const float bias = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
+      F4Features ft;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = min(feature0 + 8 * i + (lane >> 2), p.N - 1);
+        ft.h[i] = p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f;
+        ft.bias[i] = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 1700 + acc, w)))
         break;
       tc_fence_after();
@@ -403,26 +452,22 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       for (int part = 0; part < (wide ? 2 : 1); ++part) {
         const int c0 = (part == 0 ? first : 128 - first) + 32 * half;
         const bool any0 = c0 < t.nrows && feature0 < p.N, any1 = c0 + 64 < t.nrows && feature0 < p.N;
-        uint32_t r0[32], r1[32];
+        uint32_t r[4][16];
         __syncwarp();
-        if (any0) tmem_ld_x32(t_addr + (uint32_t)c0, r0);
-        if (any1) tmem_ld_x32(t_addr + (uint32_t)(c0 + 64), r1);
-        if (any0) tmem_ld_wait_dep(r0);
-        if (any1) tmem_ld_wait_dep(r1);
-        hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
-        auto factors = [&](int c) {
-          __syncwarp();
-          my_cols[lane] = p.x_scale != nullptr && c + lane < t.nrows ? p.x_scale[t.row0 + c + lane] : 1.f;
-          __syncwarp();
-        };
         if (any0) {
-          factors(c0);
-          f4_store32(p, r0, my_cols, c0, t.row0, t.nrows, feature0, h, bias, lane);
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
         }
         if (any1) {
-          factors(c0 + 64);
-          f4_store32(p, r1, my_cols, c0 + 64, t.row0, t.nrows, feature0, h, bias, lane);
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + 64u, r[2]);
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + 64u + (16u << 16), r[3]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < 2 ? any0 : any1) tmem_ld_wait_dep(r[i]);
+        hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
+        if (any0) f4_store32(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, ft, lane);
+        if (any1) f4_store32(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, ft, lane);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
@@ -474,8 +519,10 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
     auto large = [](auto kernel) {
       return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess;
     };
-    if (large(fp4_gemm_kernel<false, false>) || large(fp4_gemm_kernel<true, false>) ||
-        large(fp4_gemm_kernel<false, true>) || large(fp4_gemm_kernel<true, true>) ||
+    if (large(fp4_gemm_kernel<false, false, 1>) || large(fp4_gemm_kernel<true, false, 1>) ||
+        large(fp4_gemm_kernel<false, true, 1>) || large(fp4_gemm_kernel<true, true, 1>) ||
+        large(fp4_gemm_kernel<false, false, 2>) || large(fp4_gemm_kernel<true, false, 2>) ||
+        large(fp4_gemm_kernel<false, true, 2>) || large(fp4_gemm_kernel<true, true, 2>) ||
         cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return -3;
     attr_set[dev] = true;
@@ -514,7 +561,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   a.ldo = ldo;
   a.status = status;
   const uint64_t stage = kF4ABytes + a.b_bytes + a.sfa_bytes + a.sfb_bytes;
-  const uint64_t header = 256 + kF4EpilogueWarps * 32 * 4;
+  const uint64_t header = 256 + kF4EpilogueWarps * kF4StoreBytes;
   a.stages = (int)((227 * 1024 - header) / stage);
   if (a.stages > kF4MaxStages) a.stages = kF4MaxStages;
   const long long total = (long long)(tiles != nullptr ? max_tiles : a.m_tiles) * a.n_tiles;
@@ -547,8 +594,12 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   auto go = [&](auto kernel) {
     return launch_pdl_cluster(kernel, grid, dim3(kF4Threads), smem, stream, pair ? 2u : 1u, tw, tx, tsw, tsx, a);
   };
-  const cudaError_t e = mx ? (pair ? go(fp4_gemm_kernel<true, true>) : go(fp4_gemm_kernel<true, false>))
-                           : (pair ? go(fp4_gemm_kernel<false, true>) : go(fp4_gemm_kernel<false, false>));
+  auto wide = [&](auto one, auto two) { return a.sfb_tiles == 1 ? go(one) : go(two); };
+  const cudaError_t e =
+      mx ? (pair ? wide(fp4_gemm_kernel<true, true, 1>, fp4_gemm_kernel<true, true, 2>)
+                 : wide(fp4_gemm_kernel<true, false, 1>, fp4_gemm_kernel<true, false, 2>))
+         : (pair ? wide(fp4_gemm_kernel<false, true, 1>, fp4_gemm_kernel<false, true, 2>)
+                 : wide(fp4_gemm_kernel<false, false, 1>, fp4_gemm_kernel<false, false, 2>));
   return e == cudaSuccess ? 0 : -5;
 }
 
