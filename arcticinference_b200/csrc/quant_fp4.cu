@@ -16,10 +16,12 @@
 // function of the real numbers, whatever computes it. x / (g s) against a border of e2m1 compares an integer of
 // at most 8 bits with one of at most 7: a quotient that is no tie is at least 2^-8 away from it, relatively. It is
 // computed as x' * (1 / s) and rounded to a multiple of 2^-13 by adding and subtracting 1.5 * 2^10: the product's
-// error of 2^-22 vanishes, ties are met exactly, and all else stays on its side (a border is at least 1/4). (Which of
+// error of 2^-20 vanishes, ties are met exactly, and all else stays on its side (a border is at least 1/4). In the same
+// way max / 6 against a border of e4m3 (five bits) is rounded to fp16 first, which meets the ties and keeps the rest on
+// its side. Divisions rounded to the last bit gave the same results in twice the time. (Which of
 // its two codes a zero gets says nothing.)
 //
-// One CTA per row, the row in registers between the maximum and the rounding: one pass over memory. Eight columns
+// One CTA (or warp) per row, the row in registers between the maximum and the rounding: one pass over memory. Eight columns
 // per thread and step: 16-byte loads, 4-byte stores of codes; the lanes of a block share its maximum by shuffles and
 // four blocks' scales leave as one word. The values are the bf16 numbers that the unfused kernel would have
 // stored (same order of the norm's sum), so fused and unfused paths agree bit for bit.
@@ -52,6 +54,7 @@ struct QuantFp4Args {
   int k_tiles;
   const int4* tiles;    // optional: rows lie in these tiles (group, first row, rows), the scales by tile
   const int* num_tiles;
+  int M;
 };
 
 __device__ __forceinline__ void fq_unpack8(const uint4& q, float (&f)[8]) {
@@ -95,15 +98,16 @@ __device__ __forceinline__ uint32_t fq_block_max(uint32_t v, uint32_t* red) {
   __syncthreads();
   return __reduce_max_sync(0xffffffffu, lane < nwarps ? red[lane] : 0u);
 }
-// Eight numbers times `up` (a power of two) times `inv` -> eight codes
-__device__ __forceinline__ uint32_t fq_codes8(const uint4& raw, float up, float inv) {
+// Eight numbers times r -> eight codes. EXACT: the products are (r is a power of two).
+template <bool EXACT>
+__device__ __forceinline__ uint32_t fq_codes8(const uint4& raw, float r) {
   float v[8];
   fq_unpack8(raw, v);
-  const float2 u = make_float2(up, up), r = make_float2(inv, inv);
-  const float2 big = make_float2(1536.f, 1536.f), neg = make_float2(-1536.f, -1536.f);   // 1.5 * 2^10
+  const float2 rr = make_float2(r, r), big = make_float2(1536.f, 1536.f), neg = make_float2(-1536.f, -1536.f);   // 1.5 * 2^10
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 t = add_x2(fma_x2(mul_x2(make_float2(v[2 * i], v[2 * i + 1]), u), r, big), neg);
+    const float2 x = make_float2(v[2 * i], v[2 * i + 1]);
+    const float2 t = EXACT ? mul_x2(x, rr) : add_x2(fma_x2(x, rr, big), neg);
     v[2 * i] = t.x;
     v[2 * i + 1] = t.y;
   }
@@ -120,100 +124,157 @@ __device__ __forceinline__ uint32_t fq_codes8(const uint4& raw, float up, float 
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return w;
 }
+// Eight codes' values
+__device__ __forceinline__ void fq_values8(uint32_t w, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t"
+      ".reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t"
+      "}\n"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = t.x;
+    v[2 * i + 1] = t.y;
+  }
+}
 __device__ __forceinline__ float e4m3_value(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
 }
 
-// The place of a row's scales: the row itself, or by the tile that holds it (-1: none does).
-__device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int* found) {
+// The place of a row's scales: the row itself, or by the tile that holds it (-1: none does). A warp looks: among 32
+// tiles spread over the list, then among those from the last one that does not begin behind the row. (A tile
+// without rows fills its expert's list up to an even number and begins where the one before it ends.)
+__device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int lane) {
   if (p.tiles == nullptr) return row;
-  if (threadIdx.x == 0) *found = -1;
-  __syncthreads();
-  const int n = *p.num_tiles;
-  for (int t = threadIdx.x; t < n; t += blockDim.x) {
-    const int4 w = p.tiles[t];
-    if (row >= w.y && row < w.y + w.z) *found = t * kFp4TileRows + row - w.y;
+  const int n = *p.num_tiles, step = (n + 31) / 32;
+  bool before = false;
+  if (lane * step < n) {
+    const int4 t = p.tiles[lane * step];
+    int first = t.y;
+    if (t.z <= 0 && lane > 0) {
+      const int4 u = p.tiles[lane * step - 1];
+      first = u.y + u.z;
+    }
+    before = first <= row;
   }
-  __syncthreads();
-  return *found;
+  const uint32_t some = __ballot_sync(0xffffffffu, before);
+  if (some == 0u) return -1;
+  const int from = (31 - __clz((int)some)) * step;
+  for (int i = 0; i < step; i += 32) {
+    const int at = from + i + lane;
+    int in = -1;
+    if (i + lane < step && at < n) {
+      const int4 t = p.tiles[at];
+      if (row >= t.y && row < t.y + t.z) in = row - t.y;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, in >= 0);
+    if (hit != 0u) {
+      const int who = __ffs((int)hit) - 1;
+      return (from + i + who) * kFp4TileRows + __shfl_sync(0xffffffffu, in, who);
+    }
+  }
+  return -1;
 }
 
-template <int SRC, bool MX, int VPT>
+// WARP: a warp per row and no barrier, for rows that 32 threads hold; otherwise a block per row.
+template <int SRC, bool MX, int VPT, bool WARP>
 __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
   pdl_wait();
   pdl_trigger();
   __shared__ uint32_t red[32];
-  __shared__ int found;
+  __shared__ int block_slot;
   constexpr int kBlockVecs = MX ? 4 : 2;          // lanes of a block
   constexpr int kTileVecs = 4 * kBlockVecs;       // lanes of a word of scales
-  const int row = blockIdx.x;
+  const int lane = threadIdx.x & 31;
+  const int tid = WARP ? lane : (int)threadIdx.x, threads = WARP ? 32 : (int)blockDim.x;
+  const int row = WARP ? (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) : (int)blockIdx.x;
+  if (WARP && row >= p.M) return;
   const int nvec = p.K / 8, all = p.k_tiles * kTileVecs;
-  uint4 raw[VPT];
-  if (SRC == kFp4Silu) {
-    const int per = p.inter / 8;
-    const bf16* xr = p.x + row * p.ldx;
+  // everything that is read is requested first
+  uint4 raw[VPT], other[SRC == kFp4Plain ? 1 : VPT], wraw[SRC == kFp4Norm ? VPT : 1];
+  const uint4* xr = reinterpret_cast<const uint4*>(p.x + (long long)row * p.ldx);
+  uint4* rr = SRC == kFp4Norm && p.residual != nullptr ? reinterpret_cast<uint4*>(p.residual + (long long)row * p.K)
+                                                       : nullptr;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int i = threadIdx.x + j * blockDim.x;
-      raw[j] = make_uint4(0, 0, 0, 0);
-      if (i < nvec) {
-        const int b = p.nblk == 1 ? 0 : i / per;
-        const uint4* blk = reinterpret_cast<const uint4*>(xr + (long long)b * 2 * p.inter);
-        float g[8], u[8];
-        fq_unpack8(blk[i - b * per], g);
-        fq_unpack8(blk[per + i - b * per], u);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) g[k] = __fdividef(g[k], 1.f + __expf(-g[k])) * u[k];
-        raw[j] = fq_pack8(g);
+  for (int j = 0; j < VPT; ++j) {
+    const int i = tid + j * threads;
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (SRC != kFp4Plain) other[j] = make_uint4(0, 0, 0, 0);
+    if (SRC == kFp4Norm) wraw[j] = make_uint4(0, 0, 0, 0);
+    if (i < nvec) {
+      if (SRC == kFp4Silu) {
+        const int per = p.inter / 8, b = p.nblk == 1 ? 0 : i / per;
+        raw[j] = xr[i + b * per];
+        other[j] = xr[i + (b + 1) * per];
+      } else {
+        raw[j] = xr[i];
+        if (SRC == kFp4Norm && rr != nullptr) other[j] = rr[i];
+        if (SRC == kFp4Norm) wraw[j] = reinterpret_cast<const uint4*>(p.weight)[i];
       }
     }
-  } else {
-    const uint4* xr = reinterpret_cast<const uint4*>(p.x + row * p.ldx);
+  }
+  int slot = row;
+  if (SRC == kFp4Plain) {
+    if (WARP) {
+      slot = fq_slot(p, row, lane);
+    } else if (p.tiles != nullptr) {
+      if (threadIdx.x < 32) {
+        slot = fq_slot(p, row, lane);
+        if (lane == 0) block_slot = slot;
+      }
+      __syncthreads();
+      slot = block_slot;
+    }
+  }
+  if (SRC == kFp4Silu) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int i = threadIdx.x + j * blockDim.x;
-      raw[j] = i < nvec ? xr[i] : make_uint4(0, 0, 0, 0);
+      float g[8], u[8];
+      fq_unpack8(raw[j], g);
+      fq_unpack8(other[j], u);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = __fdividef(g[k], 1.f + __expf(-g[k])) * u[k];
+      raw[j] = fq_pack8(g);
     }
   }
   if (SRC == kFp4Norm) {
-    uint4* rr = p.residual ? reinterpret_cast<uint4*>(p.residual + (long long)row * p.K) : nullptr;
     float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int i = threadIdx.x + j * blockDim.x;
-      if (i < nvec) {
-        float v[8];
-        fq_unpack8(raw[j], v);
-        if (rr) {
-          float r[8];
-          fq_unpack8(rr[i], r);
+      const int i = tid + j * threads;
+      float v[8];
+      fq_unpack8(raw[j], v);
+      if (rr != nullptr) {
+        float a[8];
+        fq_unpack8(other[j], a);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] += r[k];
-          raw[j] = fq_pack8(v);
-          rr[i] = raw[j];
-          fq_unpack8(raw[j], v);   // normalise the value that was stored
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss += v[k] * v[k];
+        for (int k = 0; k < 8; ++k) v[k] += a[k];
+        raw[j] = fq_pack8(v);
+        if (i < nvec) rr[i] = raw[j];
+        fq_unpack8(raw[j], v);   // normalise the value that was stored
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss += v[k] * v[k];
     }
     ss = fq_block_sum(ss, reinterpret_cast<float*>(red));
     const float inv_rms = rsqrtf(ss / (float)p.K + p.eps);
-    const uint4* wr = reinterpret_cast<const uint4*>(p.weight);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int i = threadIdx.x + j * blockDim.x;
-      if (i < nvec) {
-        float v[8], w[8];
-        fq_unpack8(raw[j], v);
-        fq_unpack8(wr[i], w);
+      float v[8], f[8];
+      fq_unpack8(raw[j], v);
+      fq_unpack8(wraw[j], f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = v[k] * inv_rms * w[k];
-        raw[j] = fq_pack8(v);
-      }
+      for (int k = 0; k < 8; ++k) v[k] = v[k] * inv_rms * f[k];
+      raw[j] = fq_pack8(v);
     }
   }
-  const int slot = fq_slot(p, row, &found);
   uint32_t top[VPT], most = 0;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
@@ -225,41 +286,46 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
   }
   float up = 1.f;
   if (!MX) {
-    most = fq_block_max(most, red);
+    most = WARP ? __reduce_max_sync(0xffffffffu, most) : fq_block_max(most, red);
     // 2688 = 1.3125 * 2^11
     const uint32_t bits = most << 16;
     int e = (int)(bits >> 23) - 127 - 11 + ((bits & 0x7fffffu) > 0x280000u ? 1 : 0);
     e = most == 0 ? 0 : max(e, -126);
     const bool fine = most < 0x7f80u;
     up = fine ? fp4_pow2(-e) : 0.f;
-    if (threadIdx.x == 0 && slot >= 0) p.row_scale[row] = fine ? fp4_pow2(e) : __uint_as_float(0x7fffffffu);
+    if (tid == 0 && slot >= 0) p.row_scale[row] = fine ? fp4_pow2(e) : __uint_as_float(0x7fffffffu);
+    if (up > 0x1p+110f) {
+      // 1 / (g s) would pass the range: the row's numbers, all below 2^-98, are enlarged first (exactly)
+      up *= 0x1p-60f;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        float v[8];
+        fq_unpack8(raw[j], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= 0x1p+60f;
+        raw[j] = fq_pack8(v);
+        top[j] = __float_as_uint(__uint_as_float(top[j] << 16) * 0x1p+60f) >> 16;
+      }
+    }
   }
   if (slot < 0) return;
-  uint32_t* qr = reinterpret_cast<uint32_t*>(p.q + row * p.ldq);
+  uint32_t* qr = reinterpret_cast<uint32_t*>(p.q + (long long)row * p.ldq);
   uint8_t* sr = p.scale + (long long)(slot / kFp4TileRows) * p.k_tiles * kFp4ScaleTile +
                 fp4_scale_byte(slot % kFp4TileRows);
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int i = threadIdx.x + j * blockDim.x;
-    uint32_t byte;
-    float scaled = up, inv;
-    uint4 v = raw[j];
+    const int i = tid + j * threads;
+    uint32_t byte, code;
     if (MX) {
       const int e = max((int)(top[j] >> 7) - 2, 0);      // the exponent's field
-      byte = (uint32_t)e;
-      inv = 1.f;
-      scaled = fp4_pow2(127 - e);
-      if (top[j] >= 0x7f80u) {
-        byte = 0xffu;
-        v = make_uint4(0, 0, 0, 0);
-      }
+      byte = top[j] < 0x7f80u ? (uint32_t)e : 0xffu;
+      code = top[j] < 0x7f80u ? fq_codes8<true>(raw[j], fp4_pow2(127 - e)) : 0u;
     } else {
-      const float t = __fdiv_rn(__uint_as_float(top[j] << 16) * up, 6.f);
-      byte = most < 0x7f80u ? (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3) : 0u;
-      inv = byte ? __frcp_rn(e4m3_value(byte)) : 0.f;
-      if (byte == 0u) v = make_uint4(0, 0, 0, 0);
+      const __half t = __float2half_rn(__uint_as_float(top[j] << 16) * up * (1.f / 6.f));
+      byte = most < 0x7f80u ? (uint32_t)__nv_cvt_halfraw_to_fp8(t, __NV_SATFINITE, __NV_E4M3) : 0u;
+      code = byte != 0u ? fq_codes8<false>(raw[j], up * rcp_approx(e4m3_value(byte))) : 0u;
     }
-    if (i < nvec) qr[i] = fq_codes8(v, scaled, inv);
+    if (i < nvec) qr[i] = code;
     // the scales of four blocks in one word; blocks behind the row's end have the scale zero
     if (i >= nvec) byte = 0u;
     const uint32_t b1 = __shfl_down_sync(0xffffffffu, byte, kBlockVecs);
@@ -270,7 +336,8 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
   }
 }
 
-// One thread per eight numbers. Rows of a weight of several groups: each group's scale tiles begin anew.
+// Eight numbers per thread and step, four steps on their way together; threadIdx.y: rows of a block. Rows of a weight of
+// several groups: each group's scale tiles begin anew.
 template <bool MX>
 __global__ void __launch_bounds__(256)
 dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ scale,
@@ -281,67 +348,76 @@ dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* 
   pdl_trigger();
   constexpr int kBlockVecs = MX ? 4 : 2;
   const int nvec = K / 8;
-  auto row_of = [&](long long row, long long slot) {
+  const int padded = (group_rows + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
+  const long long items = tiles != nullptr ? (long long)*num_tiles * kFp4TileRows : rows;
+  for (long long item = (long long)blockIdx.x * blockDim.y + threadIdx.y; item < items;
+       item += (long long)gridDim.x * blockDim.y) {
+    long long row = item, slot;
+    if (tiles != nullptr) {
+      const int4 t = tiles[item / kFp4TileRows];
+      const int in = (int)(item % kFp4TileRows);
+      if (in >= t.z) continue;
+      row = t.y + in;
+      slot = item;
+    } else {
+      slot = row / group_rows * padded + row % group_rows;
+    }
     const float g = row_scale != nullptr ? row_scale[row] : 1.f;
     const uint8_t* sr = scale + slot / kFp4TileRows * k_tiles * kFp4ScaleTile +
                         fp4_scale_byte((int)(slot % kFp4TileRows));
     const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + row * ldq);
     uint4* o = reinterpret_cast<uint4*>(out + row * ldo);
-    for (int i = threadIdx.x; i < nvec; i += blockDim.x) {
-      const int b = i / kBlockVecs;
-      const uint32_t byte = sr[(long long)(b / 4) * kFp4ScaleTile + b % 4], w = qr[i];
-      float s;
-      if (MX) s = byte == 0xffu ? __uint_as_float(0x7fffffffu) : fp4_pow2((int)byte - 127);
-      else s = e4m3_value(byte);
-      float v[8];
+    for (int i0 = threadIdx.x; i0 < nvec; i0 += 4 * blockDim.x) {
+      uint32_t byte[4], w[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t c = w >> (4 * k);
-        // value of the code: (1 + m / 2) 2^(e - 1), m / 2 where e = 0
-        const int e = (int)(c >> 1) & 3;
-        const float mag = e == 0 ? 0.5f * (float)(c & 1u) : (float)(2u + (c & 1u)) * 0.25f * (float)(1 << e);
-        v[k] = ((c & 8u) ? -mag : mag) * s * g;
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * blockDim.x, b = i / kBlockVecs;
+        byte[j] = i < nvec ? sr[(long long)(b / 4) * kFp4ScaleTile + b % 4] : 0u;
+        w[j] = i < nvec ? qr[i] : 0u;
       }
-      o[i] = fq_pack8(v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * blockDim.x;
+        float s;
+        if (MX) s = byte[j] == 0xffu ? __uint_as_float(0x7fffffffu) : fp4_pow2((int)byte[j] - 127);
+        else s = e4m3_value(byte[j]);
+        float v[8];
+        fq_values8(w[j], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = v[k] * s * g;
+        if (i < nvec) o[i] = fq_pack8(v);
+      }
     }
-  };
-  if (tiles != nullptr) {
-    const int n = *num_tiles;
-    for (int t = blockIdx.x; t < n * kFp4TileRows; t += gridDim.x) {
-      const int4 w = tiles[t / kFp4TileRows];
-      const int r = t % kFp4TileRows;
-      if (r < w.z) row_of(w.y + r, t);
-    }
-    return;
   }
-  const int padded = (group_rows + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x)
-    row_of(row, row / group_rows * padded + row % group_rows);
 }
 
 template <int SRC, bool MX>
 static int launch_quant_fp4(const QuantFp4Args& a, long long M, cudaStream_t stream) {
   const int vecs = a.k_tiles * (MX ? 16 : 8);
-  // Two steps per thread keep enough loads in flight and enough threads per row; wider rows take more. (The norm's
-  // sum has the order of the unfused kernel's: 256 threads.)
-  int vpt = 1, threads = 256;
-  if (SRC == kFp4Norm) {
-    while (vpt * 256 < vecs) vpt *= 2;
-  } else {
-    while (vpt < 2 && vecs > 32 * vpt) vpt *= 2;
-    while (vecs > 512 * vpt) vpt *= 2;
-    threads = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
+  if (M > 0x7fffffff) return -6;
+  QuantFp4Args args = a;
+  args.M = (int)M;
+  auto go = [&](auto kernel, long long blocks, int threads) {
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, stream, args) == cudaSuccess ? 0 : -5;
+  };
+  if (SRC == kFp4Norm) {   // 256 threads: the norm's sum has the order of the unfused kernel's
+    if (vecs <= 256) return go(quant_fp4_kernel<SRC, MX, 1, false>, M, 256);
+    if (vecs <= 512) return go(quant_fp4_kernel<SRC, MX, 2, false>, M, 256);
+    if (vecs <= 1024) return go(quant_fp4_kernel<SRC, MX, 4, false>, M, 256);
+    return vecs <= 2048 ? go(quant_fp4_kernel<SRC, MX, 8, false>, M, 256) : -6;
   }
-  if (vpt > 8 || M > 0x7fffffff) return -6;
-  cudaError_t e;
-  const dim3 grid((unsigned)M), block((unsigned)threads);
-  switch (vpt) {
-    case 1: e = launch_pdl(quant_fp4_kernel<SRC, MX, 1>, grid, block, 0, stream, a); break;
-    case 2: e = launch_pdl(quant_fp4_kernel<SRC, MX, 2>, grid, block, 0, stream, a); break;
-    case 4: e = launch_pdl(quant_fp4_kernel<SRC, MX, 4>, grid, block, 0, stream, a); break;
-    default: e = launch_pdl(quant_fp4_kernel<SRC, MX, 8>, grid, block, 0, stream, a); break;
-  }
-  return e == cudaSuccess ? 0 : -5;
+  // Few rows want many threads each, many rows much in flight per thread (4096 columns, nvfp4, us for 2, 4 and 8
+  // steps: 128 rows 1.75, 1.89, 2.35; 8192 rows 20.2, 17.1, 16.0). The activation holds both factors: 4096 rows
+  // of 14336 62.3 with 4 steps and 110 with 8.
+  const bool many = M >= 148 * 8;
+  if (vecs <= 64) return go(quant_fp4_kernel<SRC, MX, 2, true>, (M + 3) / 4, 128);
+  if (vecs <= 128 && many) return go(quant_fp4_kernel<SRC, MX, 4, true>, (M + 3) / 4, 128);
+  int vpt = !many ? 2 : SRC == kFp4Silu ? 4 : 8;
+  while (vecs > 512 * vpt) vpt *= 2;
+  const int threads = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
+  if (vpt == 2) return go(quant_fp4_kernel<SRC, MX, 2, false>, M, threads);
+  if (vpt == 4) return go(quant_fp4_kernel<SRC, MX, 4, false>, M, threads);
+  return vpt == 8 ? go(quant_fp4_kernel<SRC, MX, 8, false>, M, threads) : -6;
 }
 
 }  // namespace ab200
@@ -356,7 +432,8 @@ extern "C" {
 
 // x bf16 [M, K], rows ldx apart -> codes [M, K / 2] (rows ldq bytes apart), scale tiles [row tiles][k_tiles][512]
 // with k_tiles = ceil(K / (4 * block)), and for nvfp4 (fmt 0; mxfp4: 1) row_scale fp32 [M]. K: a multiple of 32, at
-// most 32768. With `tiles` (int32 x 4: group, first row, rows; *num_tiles of them) a row's scales lie in
+// most 32768. With `tiles` (int32 x 4: group, first row, rows; *num_tiles of them, in
+// the order of their rows) a row's scales lie in
 // the row tile of its tile, and rows that no tile holds are left out.
 int ab200_quant_fp4(const void* x, long long ldx, void* q, long long ldq, void* scale, void* row_scale, long long M,
                     int K, int fmt, const void* tiles, const void* num_tiles, cudaStream_t stream) {
@@ -436,11 +513,11 @@ int ab200_dequant_fp4(const void* q, long long ldq, const void* scale, const voi
       (reinterpret_cast<uintptr_t>(q) & 3) || (tiles != nullptr && num_tiles == nullptr))
     return -2;
   const int nvec = K / 8;
-  const unsigned threads = nvec >= 256 ? 256u : (unsigned)((nvec + 31) / 32 * 32);
-  const long long want = rows < 148ll * 16 ? rows : 148ll * 16;
-  const dim3 grid((unsigned)(tiles != nullptr ? 148 * 8 : want));
+  const int across = nvec >= 1024 ? 256 : (((nvec + 3) / 4 + 31) / 32 * 32), down = 256 / across;
+  const long long blocks = (rows + down - 1) / down;
+  const dim3 grid((unsigned)(tiles != nullptr ? 148 * 8 : blocks < 148ll * 256 ? blocks : 148ll * 256));
   auto go = [&](auto kernel) {
-    return launch_pdl(kernel, grid, dim3(threads), 0, stream, reinterpret_cast<const uint8_t*>(q), ldq,
+    return launch_pdl(kernel, grid, dim3(across, down), 0, stream, reinterpret_cast<const uint8_t*>(q), ldq,
                       reinterpret_cast<const uint8_t*>(scale), reinterpret_cast<const float*>(row_scale),
                       reinterpret_cast<bf16*>(out), ldo, rows, K, fp4_k_tiles(K, fmt == kMxfp4), group_rows,
                       reinterpret_cast<const int4*>(tiles), reinterpret_cast<const int*>(num_tiles));
