@@ -1,6 +1,8 @@
 // torch.ops.arcticinference_b200.* : the kernels of _kernels.so as dispatcher ops, for users
 // who compose them with other PyTorch code (autograd-free, CUDA only). The engine itself calls
-// the C entry points directly (ops/native.py); both routes reach the same kernels.
+// the C entry points directly (ops/native.py); both routes reach the same kernels. The 4-bit ops
+// (fp4_*) are the exception: ops/fp4_ops.py goes through them, because their checks, allocations and
+// two launches take Python longer than the GPU needs for a step of few tokens.
 //
 // The reference registers its four kernels the same way
 // (csrc/custom_ops/torch_bindings.cpp:6-51): reshape_and_cache_flash_bulk,
@@ -300,6 +302,270 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k_cache, const at::T
   return out;
 }
 
+// ------------------------------------------------------- microscaled 4-bit numbers
+using OptTensor = c10::optional<at::Tensor>;
+
+bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+bool aligned(const at::Tensor& t, uintptr_t bytes) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0;
+}
+
+constexpr int64_t kFp4RowTile = 128, kFp4TileBytes = 512;
+
+int64_t fp4_block(int64_t fmt) {
+  TORCH_CHECK_VALUE(fmt == 0 || fmt == 1, "4-bit format ", fmt);
+  return fmt == 1 ? 32 : 16;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// bf16 rows that 16-byte accesses can read: as they are, or copied
+at::Tensor fp4_source(const at::Tensor& x, const char* what) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kBFloat16, what, ": a bf16 matrix on a GPU");
+  if (x.stride(1) == 1 && x.stride(0) % 8 == 0 && aligned(x, 16)) return x;
+  at::Tensor c = x.contiguous();
+  return aligned(c, 16) ? c : c.clone();
+}
+
+void fp4_width(int64_t K, int64_t most, const char* what) {
+  TORCH_CHECK_VALUE(K > 0 && K % 32 == 0 && K <= most, what, ": a multiple of 32 columns up to ", most, ", got ", K);
+}
+
+void on_device_of(const at::Tensor& t, const at::Tensor& o) {
+  TORCH_CHECK_VALUE(o.device() == t.device(), "tensors on ", t.device(), " and ", o.device());
+}
+void on_device_of(const at::Tensor& t, const OptTensor& o) {
+  if (has(o)) on_device_of(t, *o);
+}
+
+// Row tiles of a routing: int32 [max_tiles, 4] and how many are in use
+int64_t fp4_tiles(const at::Tensor& like, const OptTensor& tiles, const OptTensor& num) {
+  if (!has(tiles)) return 0;
+  TORCH_CHECK_VALUE(has(num) && tiles->dim() == 2 && tiles->size(1) == 4 && tiles->scalar_type() == at::kInt &&
+                        tiles->is_contiguous() && num->scalar_type() == at::kInt && num->numel() == 1,
+                    "a routing's tiles are int32 [n, 4] with their number");
+  TORCH_CHECK_VALUE(aligned(*tiles, 16), "a routing's tiles lie on a 16-byte boundary");
+  on_device_of(like, tiles);
+  on_device_of(like, num);
+  return tiles->size(0);
+}
+
+struct Fp4Out {
+  at::Tensor q, scale, row_scale;   // row_scale: without elements for mxfp4
+};
+
+Fp4Out fp4_empty(const at::Tensor& x, int64_t M, int64_t K, int64_t fmt, int64_t row_tiles) {
+  const auto bytes = x.options().dtype(at::kByte);
+  const int64_t tiles = row_tiles > 0 ? row_tiles : ceil_div(M, kFp4RowTile);
+  return {at::empty({M, K / 2}, bytes), at::empty({tiles, ceil_div(K, 4 * fp4_block(fmt)), kFp4TileBytes}, bytes),
+          at::empty({fmt == 0 ? M : 0}, x.options().dtype(at::kFloat))};
+}
+
+void* row_scale_ptr(const at::Tensor& g) { return g.numel() > 0 ? g.data_ptr() : nullptr; }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quant(const at::Tensor& x0, int64_t fmt, const OptTensor& tiles,
+                                                         const OptTensor& num_tiles) {
+  const at::Tensor x = fp4_source(x0, "quant_fp4");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1);
+  fp4_width(K, 32768, "quant_fp4");
+  Fp4Out r = fp4_empty(x, M, K, fmt, fp4_tiles(x, tiles, num_tiles));
+  if (M > 0)
+    check(ab200_quant_fp4(x.data_ptr(), x.stride(0), r.q.data_ptr(), K / 2, r.scale.data_ptr(),
+                          row_scale_ptr(r.row_scale), M, (int)K, (int)fmt, opt_ptr(tiles), opt_ptr(num_tiles),
+                          stream_of(x)),
+          "quant_fp4");
+  return {r.q, r.scale, r.row_scale};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_rmsnorm(const at::Tensor& x0, const at::Tensor& weight, double eps,
+                                                           const OptTensor& residual, int64_t fmt) {
+  const at::Tensor x = fp4_source(x0, "rmsnorm_fp4");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1);
+  fp4_width(K, 16384, "rmsnorm_fp4");
+  TORCH_CHECK_VALUE(weight.scalar_type() == at::kBFloat16 && weight.dim() == 1 && weight.size(0) == K &&
+                        weight.is_contiguous() && aligned(weight, 16),
+                    "rmsnorm_fp4: a bf16 weight of ", K);
+  on_device_of(x, weight);
+  if (has(residual)) {
+    TORCH_CHECK_VALUE(residual->scalar_type() == at::kBFloat16 && residual->sizes() == x.sizes() &&
+                          residual->is_contiguous() && aligned(*residual, 16),
+                      "rmsnorm_fp4: a contiguous bf16 residual ", x.sizes());
+    on_device_of(x, residual);
+  }
+  Fp4Out r = fp4_empty(x, M, K, fmt, 0);
+  if (M > 0)
+    check(ab200_rmsnorm_fp4(x.data_ptr(), x.stride(0), const_cast<void*>(opt_ptr(residual)), weight.data_ptr(),
+                            r.q.data_ptr(), K / 2, r.scale.data_ptr(), row_scale_ptr(r.row_scale), M, (int)K,
+                            (float)eps, (int)fmt, stream_of(x)),
+          "rmsnorm_fp4");
+  return {r.q, r.scale, r.row_scale};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_silu_mul(const at::Tensor& x0, int64_t nblk, int64_t fmt) {
+  const at::Tensor x = fp4_source(x0, "silu_mul_fp4");
+  const c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK_VALUE(nblk >= 1 && x.size(1) % (2 * nblk) == 0, "silu_mul_fp4: ", x.size(1), " columns in ", nblk,
+                    " (gate | up) blocks");
+  const int64_t M = x.size(0), K = x.size(1) / 2, inter = K / nblk;
+  fp4_width(K, 32768, "silu_mul_fp4");
+  TORCH_CHECK_VALUE(inter % 8 == 0, "silu_mul_fp4: blocks of a multiple of 8 columns, got ", inter);
+  Fp4Out r = fp4_empty(x, M, K, fmt, 0);
+  if (M > 0)
+    check(ab200_silu_mul_fp4(x.data_ptr(), x.stride(0), r.q.data_ptr(), K / 2, r.scale.data_ptr(),
+                             row_scale_ptr(r.row_scale), M, (int)inter, (int)nblk, (int)fmt, stream_of(x)),
+          "silu_mul_fp4");
+  return {r.q, r.scale, r.row_scale};
+}
+
+// Codes and scale tiles of one matrix or several, and the factors of their rows
+struct Fp4Operand {
+  int64_t groups, rows, K;
+};
+Fp4Operand fp4_operand(const at::Tensor& q, const at::Tensor& scale, const OptTensor& row_scale, int64_t fmt,
+                       int64_t row_tiles, const char* what) {
+  TORCH_CHECK_VALUE(q.is_cuda() && q.scalar_type() == at::kByte && (q.dim() == 2 || q.dim() == 3) && q.stride(-1) == 1 &&
+                        q.size(-1) % 16 == 0,
+                    what, ": codes are uint8 [.., rows, K / 2] with K a multiple of 32");
+  Fp4Operand o = {q.dim() == 3 ? q.size(0) : 1, q.size(-2), 2 * q.size(-1)};
+  bool ok = q.stride(-2) % 16 == 0 && aligned(q, 16);
+  if (q.dim() == 3) ok = ok && q.stride(0) % 16 == 0;
+  TORCH_CHECK_VALUE(ok, what, ": rows of codes on 16-byte boundaries");
+  TORCH_CHECK_VALUE(scale.scalar_type() == at::kByte && scale.is_contiguous() && aligned(scale, 16) &&
+                        scale.dim() == q.dim() + 1 && scale.size(-1) == kFp4TileBytes &&
+                        scale.size(-2) == ceil_div(o.K, 4 * fp4_block(fmt)) &&
+                        scale.size(-3) == (row_tiles > 0 ? row_tiles : ceil_div(o.rows, kFp4RowTile)) &&
+                        (q.dim() == 2 || scale.size(0) == o.groups),
+                    what, ": scale tiles ", scale.sizes(), " do not belong to codes ", q.sizes());
+  on_device_of(q, scale);
+  if (has(row_scale)) {
+    TORCH_CHECK_VALUE(row_scale->scalar_type() == at::kFloat && row_scale->is_contiguous() &&
+                          row_scale->numel() == o.groups * o.rows,
+                      what, ": a contiguous fp32 factor per row");
+    on_device_of(q, row_scale);
+  }
+  return o;
+}
+
+void fp4_dequant(const at::Tensor& q, const at::Tensor& scale, const OptTensor& row_scale, int64_t fmt,
+                 const OptTensor& tiles, const OptTensor& num_tiles, at::Tensor out) {
+  const int64_t row_tiles = fp4_tiles(q, tiles, num_tiles);
+  const Fp4Operand o = fp4_operand(q, scale, row_scale, fmt, row_tiles, "dequant_fp4");
+  TORCH_CHECK_VALUE(q.dim() == 2 || q.stride(0) == q.stride(1) * q.size(1), "dequant_fp4: matrices behind one another");
+  TORCH_CHECK_VALUE(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == q.dim() &&
+                        out.size(-1) == o.K && out.size(-2) == o.rows && (q.dim() == 2 || out.size(0) == o.groups) &&
+                        aligned(out, 16),
+                    "dequant_fp4: out is a contiguous bf16 tensor of the rows' shape");
+  on_device_of(q, out);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t R = o.groups * o.rows;
+  if (R > 0 && o.K > 0)
+    check(ab200_dequant_fp4(q.data_ptr(), q.stride(-2), scale.data_ptr(), opt_ptr(row_scale), out.data_ptr(), o.K, R,
+                            (int)o.K, (int)o.rows, (int)fmt, opt_ptr(tiles), opt_ptr(num_tiles), stream_of(q)),
+          "dequant_fp4");
+}
+
+// x: bf16 rows, quantised here into scratch, or xq, xs, xg
+void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
+                 const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt, const OptTensor& bias,
+                 const OptTensor& residual, int64_t act, int64_t gate, double limit, double alpha,
+                 const OptTensor& tiles, const OptTensor& num_tiles, at::Tensor& out, const at::Tensor& status) {
+  const int64_t row_tiles = fp4_tiles(wq, tiles, num_tiles);
+  const Fp4Operand w = fp4_operand(wq, ws, wg, fmt, 0, "4-bit weight");
+  const c10::cuda::CUDAGuard guard(wq.device());
+  const cudaStream_t stream = stream_of(wq);
+  const int64_t N = w.rows, K = w.K;
+  at::Tensor x, scratch;
+  const void *q, *s, *g;
+  int64_t M, ldx;
+  if (has(x0)) {
+    x = fp4_source(*x0, "4-bit product");
+    M = x.size(0);
+    on_device_of(wq, x);
+    TORCH_CHECK_VALUE(x.size(1) == K, "4-bit product: rows of ", x.size(1), " columns and a weight of ", K);
+    fp4_width(K, 32768, "quant_fp4");
+  } else {
+    TORCH_CHECK_VALUE(has(xq) && has(xs), "4-bit product: rows are missing");
+    const Fp4Operand o = fp4_operand(*xq, *xs, xg, fmt, row_tiles, "4-bit rows");
+    TORCH_CHECK_VALUE(o.groups == 1 && xq->dim() == 2 && o.K == K, "4-bit product: rows ", xq->sizes(), " and weight ",
+                      wq.sizes());
+    on_device_of(wq, xq);
+    M = o.rows;
+  }
+  const bool grouped = row_tiles > 0;
+  TORCH_CHECK_VALUE(grouped == (wq.dim() == 3), "4-bit product: several matrices go with a routing");
+  TORCH_CHECK_VALUE(N % (gate ? 32 : 8) == 0, "4-bit product: N a multiple of ", gate ? 32 : 8, ", got ", N);
+  const int64_t width = gate ? N / 2 : N;
+  auto matrix = [&](const at::Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.size(0) == M && t.size(1) == width, "4-bit product: ",
+                      what, " is bf16 [", M, ", ", width, "]");
+    TORCH_CHECK_VALUE(t.stride(1) == 1 && t.stride(0) % 8 == 0 && aligned(t, 16), "4-bit product: rows of ", what,
+                      " on 16-byte boundaries");
+    on_device_of(wq, t);
+  };
+  if (has(residual)) matrix(*residual, "residual");
+  if (has(bias)) {
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kBFloat16 && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous(),
+                      "4-bit product: bias is bf16 [", N, "]");
+    on_device_of(wq, bias);
+  }
+  if (out.defined()) matrix(out, "out");
+  else out = at::empty({M, width}, wq.options().dtype(at::kBFloat16));
+  if (M == 0 || N == 0) return;
+  if (has(x0)) {
+    const int64_t k_tiles = ceil_div(K, 4 * fp4_block(fmt));
+    const int64_t codes = ceil_div(M * K / 2, 512) * 512;
+    const int64_t scales = (grouped ? row_tiles : ceil_div(M, kFp4RowTile)) * k_tiles * kFp4TileBytes;
+    scratch = at::empty({codes + scales + (fmt == 0 ? 4 * M : 0)}, wq.options());
+    uint8_t* base = scratch.data_ptr<uint8_t>();
+    q = base;
+    s = base + codes;
+    g = fmt == 0 ? base + codes + scales : nullptr;
+    ldx = K / 2;
+    check(ab200_quant_fp4(x.data_ptr(), x.stride(0), base, ldx, base + codes, const_cast<void*>(g), M, (int)K, (int)fmt,
+                          opt_ptr(tiles), opt_ptr(num_tiles), stream),
+          "quant_fp4");
+  } else {
+    q = xq->data_ptr();
+    s = xs->data_ptr();
+    g = opt_ptr(xg);
+    ldx = xq->stride(0);
+  }
+  check(ab200_linear_fp4(q, ldx, s, g, wq.data_ptr(), wq.stride(-2), wq.dim() == 3 ? wq.stride(0) : 0, ws.data_ptr(),
+                         opt_ptr(wg), out.data_ptr(), out.stride(0), M, (int)N, (int)K, (int)w.groups, (int)fmt,
+                         opt_ptr(bias), opt_ptr(residual), has(residual) ? residual->stride(0) : 0, (int)act, (int)gate,
+                         (float)limit, (float)alpha, opt_ptr(tiles), opt_ptr(num_tiles), (int)row_tiles,
+                         status.data_ptr<int>(), stream),
+        "linear_fp4");
+}
+
+at::Tensor fp4_linear(const OptTensor& x, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
+                      const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt,
+                      const OptTensor& bias, const OptTensor& residual, int64_t act, const at::Tensor& status) {
+  at::Tensor out;
+  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, bias, residual, act, 0, 0, 0, {}, {}, out, status);
+  return out;
+}
+
+void fp4_linear_out(const OptTensor& x, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
+                    const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt,
+                    const OptTensor& bias, const OptTensor& residual, int64_t act, const at::Tensor& status,
+                    at::Tensor out) {
+  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, bias, residual, act, 0, 0, 0, {}, {}, out, status);
+}
+
+at::Tensor fp4_grouped_linear(const OptTensor& x, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
+                              const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt,
+                              const at::Tensor& tiles, const at::Tensor& num_tiles, int64_t gate, double limit,
+                              double alpha, const at::Tensor& status) {
+  TORCH_CHECK_VALUE(wq.dim() == 3, "grouped_linear_fp4: weights [E, N, K]");
+  at::Tensor out;
+  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, {}, {}, 0, gate, limit, alpha, tiles, num_tiles, out, status);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(arcticinference_b200, m) {
@@ -328,6 +594,17 @@ TORCH_LIBRARY(arcticinference_b200, m) {
   m.def("attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor work, "
         "Tensor tok_splits, int max_splits, int Hq, int Hkv, int D, bool causal, float scale, "
         "int tile_keys=128) -> Tensor");
+  m.def("fp4_quant(Tensor x, int fmt, Tensor? tiles=None, Tensor? num_tiles=None) -> (Tensor, Tensor, Tensor)");
+  m.def("fp4_rmsnorm(Tensor x, Tensor weight, float eps, Tensor(a!)? residual, int fmt) -> (Tensor, Tensor, Tensor)");
+  m.def("fp4_silu_mul(Tensor x, int nblk, int fmt) -> (Tensor, Tensor, Tensor)");
+  m.def("fp4_dequant(Tensor q, Tensor scale, Tensor? row_scale, int fmt, Tensor? tiles, Tensor? num_tiles, "
+        "Tensor(a!) out) -> ()");
+  m.def("fp4_linear(Tensor? x, Tensor? xq, Tensor? xs, Tensor? xg, Tensor wq, Tensor ws, Tensor? wg, int fmt, "
+        "Tensor? bias, Tensor? residual, int act, Tensor status) -> Tensor");
+  m.def("fp4_linear_out(Tensor? x, Tensor? xq, Tensor? xs, Tensor? xg, Tensor wq, Tensor ws, Tensor? wg, int fmt, "
+        "Tensor? bias, Tensor? residual, int act, Tensor status, Tensor(a!) out) -> ()");
+  m.def("fp4_grouped_linear(Tensor? x, Tensor? xq, Tensor? xs, Tensor? xg, Tensor wq, Tensor ws, Tensor? wg, int fmt, "
+        "Tensor tiles, Tensor num_tiles, int gate, float limit, float alpha, Tensor status) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(arcticinference_b200, CUDA, m) {
@@ -345,4 +622,11 @@ TORCH_LIBRARY_IMPL(arcticinference_b200, CUDA, m) {
   m.impl("linear_fp8_row", &linear_fp8_row);
   m.impl("rope_cache", &rope_cache);
   m.impl("attention", &attention);
+  m.impl("fp4_quant", &fp4_quant);
+  m.impl("fp4_rmsnorm", &fp4_rmsnorm);
+  m.impl("fp4_silu_mul", &fp4_silu_mul);
+  m.impl("fp4_dequant", &fp4_dequant);
+  m.impl("fp4_linear", &fp4_linear);
+  m.impl("fp4_linear_out", &fp4_linear_out);
+  m.impl("fp4_grouped_linear", &fp4_grouped_linear);
 }

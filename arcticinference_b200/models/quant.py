@@ -373,23 +373,31 @@ class Fp4Rows:
     __slots__ = ("q", "scale", "row_scale", "fmt", "routing")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, row_scale, fmt: str, routing=None):
-        check_fp4_format(fmt)
-        if q.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        size = FP4_BLOCK.get(fmt)
+        if size is None:
+            check_fp4_format(fmt)
+        if q.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
             raise ValueError("4-bit codes and scales are uint8 tensors")
-        if q.dim() not in (2, 3) or q.shape[-1] % 16:
-            raise ValueError("4-bit codes: [rows, K / 2] with K a multiple of 32, got %s" % (tuple(q.shape),))
-        tiles = fp4_scale_tiles(q.shape[-2], 2 * q.shape[-1], fmt)
-        if routing is not None:
-            tiles = (scale.shape[-3],) + tiles[1:]
-        if tuple(scale.shape) != tuple(q.shape[:-2]) + tiles:
-            raise ValueError("scale tiles %s do not belong to codes %s" % (tuple(scale.shape), tuple(q.shape)))
-        if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != q.shape[:-1]):
-            raise ValueError("row factors: fp32 %s" % (tuple(q.shape[:-1]),))
+        a, b = q.shape, scale.shape
+        if not 2 <= len(a) <= 3 or a[-1] % 16:
+            raise ValueError("4-bit codes: [rows, K / 2] with K a multiple of 32, got %s" % (tuple(a),))
+        if len(b) != len(a) + 1 or b[-1] != FP4_TILE_BYTES or b[-2] != -(-a[-1] // (2 * size)) or \
+                (routing is None and b[-3] != -(-a[-2] // FP4_ROW_TILE)) or (len(a) == 3 and a[0] != b[0]):
+            raise ValueError("scale tiles %s do not belong to codes %s" % (tuple(b), tuple(a)))
+        if row_scale is not None and (row_scale.dtype is not torch.float32 or row_scale.shape != a[:-1]):
+            raise ValueError("row factors: fp32 %s" % (tuple(a[:-1]),))
         self.q = q
         self.scale = scale
         self.row_scale = row_scale
         self.fmt = fmt
         self.routing = routing
+
+    @classmethod
+    def _of(cls, q, scale, row_scale, fmt, routing):
+        """What an operator has made: nothing to check."""
+        r = cls.__new__(cls)
+        r.q, r.scale, r.row_scale, r.fmt, r.routing = q, scale, row_scale, fmt, routing
+        return r
 
     @property
     def shape(self):

@@ -157,12 +157,6 @@ def _declare(L: ctypes.CDLL) -> None:
                                    F, I, P, P]),
         "ab200_latent_attention": (I, [P, LL, P, I, I, P, I, P, I, P, I, LL, I, I, I, I, I, I, F, P, P,
                                        LL, P, P, P, P, P]),
-        "ab200_quant_fp4": (I, [P, LL, P, LL, P, P, LL, I, I, P, P, P]),
-        "ab200_rmsnorm_fp4": (I, [P, LL, P, P, P, LL, P, P, LL, I, F, I, P]),
-        "ab200_silu_mul_fp4": (I, [P, LL, P, LL, P, P, LL, I, I, I, P]),
-        "ab200_dequant_fp4": (I, [P, LL, P, P, P, LL, LL, I, I, I, P, P, P]),
-        "ab200_linear_fp4": (I, [P, LL, P, P, P, LL, LL, P, P, P, LL, LL, I, I, I, I, P, P, LL, I, I, F, F, P, P, I, P,
-                                 P]),
         "ab200_attention_ext": (I, [P, LL, P, P, LL, LL, I, P, I, P, I, P, I, LL, I, I, I, I, I, I, P,
                                     P, LL, I, F, F, P, LL, P, P, I, P, P]),
         "ab200_attention": (I, [P, LL, P, P, LL, LL, I, P, I, P, I, P, I, LL, I, I, I, I, F, P,
