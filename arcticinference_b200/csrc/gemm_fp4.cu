@@ -8,7 +8,7 @@
 // Features are the tensor core's M side (128 per CTA), tokens its N side: a step's instruction is as wide as
 // there are tokens, so a single token or a ragged group costs what it has. One thread feeds a ring of stages by TMA:
 // 256 columns of both operands (128 bytes a row, 128-byte swizzle) and their scale tiles. One warp copies a stage's
-// scales to tensor memory (two sets, used in turn) and issues the products into one of two accumulators;
+// scales to tensor memory (sets used in turn) and issues the products into one of two accumulators;
 // eight warps drain the other one.
 
 #include <stdlib.h>
@@ -30,9 +30,9 @@ constexpr int kF4MaxStages = 10;
 constexpr int kF4StoreBytes = 32 * 64;                 // a warp's staging tile
 constexpr int kF4StepCols = 256;                       // columns of a stage: 128 bytes of codes
 constexpr uint32_t kF4ABytes = 128 * 128;
-// Tensor memory: columns 0 - 383 for two accumulators, then two sets of scales. An accumulator of more than 128 tokens
+// Tensor memory: columns 0 - 383 for two accumulators, then sets of scales. An accumulator of more than 128 tokens
 // takes columns 0 - 255 or 128 - 383: the middle ones belong to both, are drained first and handed on at once.
-constexpr uint32_t kF4Middle = 128, kF4ScaleAt = 384, kF4ScaleSet = 64;
+constexpr uint32_t kF4Middle = 128, kF4ScaleAt = 384;
 constexpr int kF4MaxTokens = 256;
 
 struct Fp4GemmArgs {
@@ -338,10 +338,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       constexpr uint32_t kSfaBytes = kTiles * kFp4ScaleTile;
       int stage = 0, acc = 0;
       uint32_t phase = 0, side_phase = 0, middle_phase = 0;
-      // the stages of the last step and of the one before: its products must be done before its set of scales is
-      // written again
-      int last_stage = -1, old_stage = -1;
-      uint32_t last_phase = 0, old_phase = 0, set = 0;
+      // A step's scales go to one of two or four sets in turn: the products that read the set last must be done.
+      constexpr int kSets = SFB == 1 ? 4 : 2;
+      constexpr uint32_t kSetColumns = 128u / kSets;
+      uint32_t set = 0;
+      int steps = 0;
       bool ok = true;
       for (int w = first_work; w < total_work && ok; w += work_step) {
         const F4Work t = f4_work(p, w);
@@ -359,10 +360,13 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         const uint32_t idesc = make_idesc_fp4(128 * kCtas, n, MX, 0), idesc_hi = make_idesc_fp4(128 * kCtas, n, MX, 2);
         const uint32_t d_tmem = __shfl_sync(0xffffffffu, tm + f4_accumulator(acc, t.nrows), 0);
         for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (old_stage >= 0 && !__all_sync(0xffffffffu, mbar_wait(empty_bar(old_stage), old_phase, abort_flag,
-                                                                   p.status, 1620 + stage, kb))) {
-            ok = false;
-            break;
+          if (steps >= kSets) {
+            const bool wrapped = stage < kSets;
+            if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage - kSets + (wrapped ? p.stages : 0)),
+                                                   phase ^ (wrapped ? 1u : 0u), abort_flag, p.status, 1620 + stage, kb))) {
+              ok = false;
+              break;
+            }
           }
           if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.status, 1640 + stage, kb))) {
             ok = false;
@@ -373,7 +377,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
           const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
           const uint64_t sb_desc = sa_desc + (uint64_t)(kSfaBytes / 16);
-          const uint32_t sfa = tm + kF4ScaleAt + set * kF4ScaleSet, sfb = sfa + 16u;
+          const uint32_t sfa = tm + kF4ScaleAt + set * kSetColumns, sfb = sfa + 16u;
           const uint32_t sfb_first = sfb + shift;
           if (elect_one()) {
 #pragma unroll
@@ -400,11 +404,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
             }
           }
           __syncwarp();
-          old_stage = last_stage;
-          old_phase = last_phase;
-          last_stage = stage;
-          last_phase = phase;
-          set ^= 1u;
+          set = set + 1u == (uint32_t)kSets ? 0u : set + 1u;
+          ++steps;
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1u;
@@ -484,6 +485,283 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   }
 }
 
+// ------------------------------------------------------------------------------------------
+// Few tokens (at most 256): the weights are streamed once, which bounds it. A CTA has 128 features and, where these
+// tiles are fewer than the SMs, a part of K: the CTAs of a cluster that share a tile exchange their fp32 sums
+// through shared memory, slices of 16 features, and each adds those of its own slices in the order of K and stores
+// them. The weights' first steps are requested into L2 before the wait for the kernel ahead, whose tail (the rows'
+// quantisation) they cover: a prefetch changes no value, whoever has written them.
+struct Fp4FewArgs {
+  int N, M, kblocks, splits, per_split, stages;
+  uint32_t b_bytes, columns, scale_at;
+  int act;
+  const float* x_scale;
+  const float* w_scale;
+  const bf16* bias;
+  const bf16* residual;
+  long long ldr;
+  bf16* out;
+  long long ldo;
+  int* status;
+};
+
+constexpr int kFewSlice = 16;                    // features of an exchanged slice
+constexpr uint32_t kFewHeader = 1024;            // barriers in front of the stages
+// Tensor memory: the accumulator, then a set of scales per stage, so that a stage's wait covers its set too. A set of
+// its own for every second step only (as in the kernel above) made a step wait for the one before the last: 0.33
+// instead of 0.15 us a step for one token.
+constexpr uint32_t few_scale_set(int sfb) { return 16u + 16u * (uint32_t)sfb; }
+
+__device__ __forceinline__ void tma_prefetch_3d(const void* tmap, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void st_cluster_v2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+
+template <bool MX, int SFB>
+__global__ void __launch_bounds__(kF4Threads, SFB == 1 ? 2 : 1)
+fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+               const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
+               const Fp4FewArgs p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
+    pdl_trigger();
+    pdl_wait();
+    if (threadIdx.x == 0) report_error(p.status, kErrBadArgument, 1800, (int)(smem_u32(smem) & 1023u));
+    return;
+  }
+  constexpr int kTiles = MX ? 2 : 4;
+  constexpr uint32_t kSfaBytes = kTiles * kFp4ScaleTile;
+  const uint32_t stage_bytes = kF4ABytes + p.b_bytes + kSfaBytes * (1 + SFB);
+  const uint32_t base = smem_u32(smem);
+  const uint32_t stages0 = base + kFewHeader;
+  auto full_bar = [&](int s) { return base + 8u * s; };
+  auto empty_bar = [&](int s) { return base + 8u * (kF4MaxStages + s); };
+  const uint32_t done_bar = base + 8u * (2 * kF4MaxStages);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 8 * (2 * kF4MaxStages + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* ring = smem + kFewHeader;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int tile = (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits;
+  const int k0 = split * p.per_split, n = min(p.per_split, p.kblocks - k0);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    const int ahead = min(n, 2 * p.stages);
+    for (int i = 0; i < ahead; ++i) {
+      tma_prefetch_3d(&tmap_w, (k0 + i) * 128, tile * 128, 0);
+      tma_prefetch_3d(&tmap_sw, 0, (k0 + i) * kTiles, tile);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), p.columns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();   // (tensor memory is owned)
+  pdl_wait();
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 1;
+      for (int i = 0; i < n; ++i) {
+        if (!mbar_wait(empty_bar(stage), phase, abort_flag, p.status, 1800 + stage, i)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(full_bar(stage), stage_bytes);
+        const uint32_t dst = stages0 + (uint32_t)stage * stage_bytes;
+        const uint32_t sfa = dst + kF4ABytes + p.b_bytes;
+        tma_load_3d(dst, &tmap_w, full_bar(stage), (k0 + i) * 128, tile * 128, 0);
+        tma_load_3d(sfa, &tmap_sw, full_bar(stage), 0, (k0 + i) * kTiles, tile);
+        tma_load_2d(dst + kF4ABytes, &tmap_x, full_bar(stage), (k0 + i) * 128, 0);
+        tma_load_3d(sfa + kSfaBytes, &tmap_sx, full_bar(stage), 0, (k0 + i) * kTiles, 0);
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) {   // copies already issued get a short time to land
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 20000000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
+    const uint64_t a0 = make_desc_kmajor_sw128(stages0);
+    const uint64_t s0 = make_desc_scales(stages0 + kF4ABytes + p.b_bytes);
+    const uint64_t stage_step = stage_bytes / 16;
+    const uint32_t width = (uint32_t)f4_width(p.M);
+    const uint32_t idesc = make_idesc_fp4(128, width, MX, 0), idesc_hi = make_idesc_fp4(128, width, MX, 2);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < n; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag, p.status, 1840 + stage, i))) break;
+      tc_fence_after();
+      const uint64_t a_desc = a0 + (uint64_t)stage * stage_step;
+      const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
+      const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
+      const uint64_t sb_desc = sa_desc + (uint64_t)(kSfaBytes / 16);
+      const uint32_t sfa = tm + p.scale_at + (uint32_t)stage * few_scale_set(SFB), sfb = sfa + 16u;
+      if (elect_one()) {
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          tmem_copy_scales<false>(sfa + 4u * j, sa_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
+#pragma unroll
+          for (int q = 0; q < SFB; ++q)
+            tmem_copy_scales<false>(sfb + 4u * (SFB * j + q),
+                                    sb_desc + (uint64_t)((q * kTiles + j) * (kFp4ScaleTile / 16)));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = MX ? k / 2 : k;
+          umma_fp4_ss<MX, false>(tm, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
+                                 MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j, sfb + 4u * SFB * j,
+                                 (i > 0 || k > 0) ? 1u : 0u);
+        }
+        tc_commit(empty_bar(stage));
+        if (i == n - 1) tc_commit(done_bar);
+      }
+      __syncwarp();
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  }
+  const int quad = warp & 3, half = (warp - 2) >> 2;
+  const uint32_t t_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
+  if (p.splits == 1) {
+    if (warp >= 2) {
+      const int feature0 = tile * 128 + quad * 32;
+      F4Features ft;
+      Fp4GemmArgs g = {};
+      g.N = p.N;
+      g.act = p.act;
+      g.x_scale = p.x_scale;
+      g.residual = p.residual;
+      g.ldr = p.ldr;
+      g.out = p.out;
+      g.ldo = p.ldo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = min(feature0 + 8 * i + (lane >> 2), p.N - 1);
+        ft.h[i] = p.w_scale != nullptr ? p.w_scale[f] : 1.f;
+        ft.bias[i] = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.status, 1900, n));
+      tc_fence_after();
+      if (ok && feature0 < p.N)
+        for (int c0 = 32 * half; c0 < p.M; c0 += 64) {
+          uint32_t lo[16], hi[16];
+          __syncwarp();
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0, lo);
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), hi);
+          tmem_ld_wait_dep(lo);
+          tmem_ld_wait_dep(hi);
+          f4_store32(g, lo, hi, ring + (warp - 2) * kF4StoreBytes, c0, 0, p.M, feature0, ft, lane);
+        }
+    }
+  } else {
+    // [source][slice of this CTA][16 features][tokens] floats where the stages were
+    const int pitch = ((p.M + 31) & ~31) + 8, mine = 8 / p.splits;
+    const uint32_t slice_bytes = (uint32_t)(kFewSlice * pitch) * 4u, source_bytes = slice_bytes * (uint32_t)mine;
+    const uint32_t my = cluster_ctarank();
+    if (warp >= 2) {
+      ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.status, 1900, n));
+      tc_fence_after();
+    }
+    __syncthreads();
+    cluster_sync();   // every CTA of the cluster has read its last stage
+    if (warp >= 2 && ok) {
+      for (int c0 = 32 * half; c0 < p.M; c0 += 64) {
+        uint32_t r[2][16];
+        __syncwarp();
+        tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
+        tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
+        tmem_ld_wait_dep(r[0]);
+        tmem_ld_wait_dep(r[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int slice = 2 * quad + h;
+          const uint32_t to = map_to_cta(stages0 + my * source_bytes + (uint32_t)(slice % mine) * slice_bytes +
+                                             (uint32_t)((lane >> 2) * pitch + c0 + 2 * (lane & 3)) * 4u,
+                                         (uint32_t)(slice / mine));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c0 + 8 * j < p.M) {
+              st_cluster_v2(to + 32u * j, r[h][4 * j], r[h][4 * j + 1]);
+              st_cluster_v2(to + 32u * j + 32u * (uint32_t)pitch, r[h][4 * j + 2], r[h][4 * j + 3]);
+            }
+        }
+      }
+    }
+    cluster_sync();
+    if (warp >= 2 && ok) {
+      // eight features of a token each
+      const int items = 2 * mine * p.M;
+      for (int it = (int)threadIdx.x - 64; it < items; it += kF4EpilogueWarps * 32) {
+        const int part = it / p.M, m = it - part * p.M;
+        const int f = tile * 128 + (int)my * mine * kFewSlice + 8 * part;
+        if (f >= p.N) continue;
+        const float* at = reinterpret_cast<const float*>(ring) + (size_t)(8 * part) * pitch + m;
+        const float gx = p.x_scale != nullptr ? p.x_scale[m] : 1.f;
+        uint4 rq = make_uint4(0, 0, 0, 0);
+        if (p.residual != nullptr) rq = *reinterpret_cast<const uint4*>(p.residual + (long long)m * p.ldr + f);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int src = 0; src < p.splits; ++src) {
+          const float* a = at + (size_t)src * (source_bytes / 4);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += a[e * pitch];
+        }
+        const __nv_bfloat162* rp = reinterpret_cast<const __nv_bfloat162*>(&rq);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float h = p.w_scale != nullptr ? p.w_scale[f + e] : 1.f;
+          v[e] = v[e] * (gx * h) + (p.bias != nullptr ? __bfloat162float(p.bias[f + e]) : 0.f);
+          if (p.act == 1) v[e] = gelu_exact(v[e]);
+        }
+        if (p.residual != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 t = __bfloat1622float2(rp[e]);
+            v[2 * e] += t.x;
+            v[2 * e + 1] += t.y;
+          }
+        }
+        *reinterpret_cast<uint4*>(p.out + (long long)m * p.ldo + f) =
+            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                       pack_bf16x2(v[6], v[7]));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, p.columns);
+  }
+}
+
 }  // namespace ab200
 
 using namespace ab200;
@@ -523,16 +801,90 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
         large(fp4_gemm_kernel<false, true, 1>) || large(fp4_gemm_kernel<true, true, 1>) ||
         large(fp4_gemm_kernel<false, false, 2>) || large(fp4_gemm_kernel<true, false, 2>) ||
         large(fp4_gemm_kernel<false, true, 2>) || large(fp4_gemm_kernel<true, true, 2>) ||
+        large(fp4_few_kernel<false, 1>) || large(fp4_few_kernel<true, 1>) || large(fp4_few_kernel<false, 2>) ||
+        large(fp4_few_kernel<true, 2>) ||
         cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return -3;
     attr_set[dev] = true;
   }
   const int sms = sm_count[dev];
+  const int step_tiles = mx ? 2 : 4, kblocks = (K + kF4StepCols - 1) / kF4StepCols;
+  const int w_row_tiles = (N + 127) / 128, k_tiles = fp4_k_tiles(K, mx);
+  CUtensorMap tw, tx, tsw, tsx;
+  // tokens of a tile (their rows of codes per CTA), row tiles that their scales lie in
+  auto make_maps = [&](int x_rows, int sfb_tiles) {
+    const uint64_t dims[3] = {(uint64_t)K / 2, (uint64_t)N, (uint64_t)groups};
+    const uint64_t strides[2] = {(uint64_t)ldw, (uint64_t)(groups > 1 ? w_gstride : ldw)};
+    const uint32_t box[3] = {128, 128, 1};
+    auto scales = [&](CUtensorMap* map, const void* base, uint64_t row_tiles, uint32_t box_tiles) {
+      const uint64_t sdims[3] = {kFp4ScaleTile / 4, (uint64_t)k_tiles, row_tiles};
+      const uint64_t sstrides[2] = {kFp4ScaleTile, (uint64_t)k_tiles * kFp4ScaleTile};
+      const uint32_t sbox[3] = {kFp4ScaleTile / 4, (uint32_t)step_tiles, box_tiles};
+      return make_tmap_nd(map, base, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, sdims, sstrides, sbox,
+                          CU_TENSOR_MAP_SWIZZLE_NONE);
+    };
+    return make_tmap_nd(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, dims, strides, box) == 0 &&
+           make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K / 2, (uint64_t)ldx,
+                        (uint32_t)x_rows, 128) == 0 &&
+           scales(&tsw, sw, (uint64_t)groups * w_row_tiles, 1) == 0 &&
+           scales(&tsx, sx, (uint64_t)(tiles != nullptr ? max_tiles : (M + 127) / 128), (uint32_t)sfb_tiles) == 0;
+  };
+
+  if (tiles == nullptr && M <= (getenv("F4_FEW") ? atoi(getenv("F4_FEW")) : 256)) {
+    Fp4FewArgs f;
+    memset(&f, 0, sizeof(f));
+    f.N = N;
+    f.M = (int)M;
+    f.kblocks = kblocks;
+    const int x_rows = (int)(M + 15) / 16 * 16, sfb = M > 128 ? 2 : 1;
+    f.b_bytes = (uint32_t)x_rows * 128;
+    const uint64_t stage = kF4ABytes + f.b_bytes + (uint64_t)step_tiles * kFp4ScaleTile * (1 + sfb);
+    // More tiles than SMs: two CTAs on each, with half of its shared and tensor memory (for up to 128 tokens). Fewer: a
+    // tile's steps are split.
+    const int per_sm = sfb == 1 && w_row_tiles > sms ? 2 : 1;
+    f.splits = 1;
+    while (f.splits < 8 && w_row_tiles * f.splits * 2 <= sms && kblocks >= 2 * f.splits) f.splits *= 2;
+    if (getenv("F4_SPLITS")) f.splits = atoi(getenv("F4_SPLITS"));
+    f.per_split = (kblocks + f.splits - 1) / f.splits;
+    while (f.splits > 1 && f.per_split * (f.splits - 1) >= kblocks) {   // every CTA of a cluster has work
+      f.splits /= 2;
+      f.per_split = (kblocks + f.splits - 1) / f.splits;
+    }
+    const uint64_t exchange =
+        f.splits > 1 ? (uint64_t)8 * kFewSlice * (((M + 31) & ~31ll) + 8) * 4 : kF4EpilogueWarps * kF4StoreBytes;
+    f.columns = per_sm == 2 ? 256 : 512;
+    f.scale_at = M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    const int sets = (int)((f.columns - f.scale_at) / few_scale_set(sfb));
+    f.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - kFewHeader) / stage);
+    if (f.stages > kF4MaxStages) f.stages = kF4MaxStages;
+    if (f.stages > sets) f.stages = sets;
+    if (f.stages > f.per_split) f.stages = f.per_split;
+    uint64_t body = f.stages * stage;
+    if (body < exchange) body = exchange;
+    f.act = act;
+    f.x_scale = reinterpret_cast<const float*>(gx);
+    f.w_scale = reinterpret_cast<const float*>(gw);
+    f.bias = reinterpret_cast<const bf16*>(bias);
+    f.residual = reinterpret_cast<const bf16*>(residual);
+    f.ldr = ldr;
+    f.out = reinterpret_cast<bf16*>(out);
+    f.ldo = ldo;
+    f.status = status;
+    if (!make_maps(x_rows, sfb)) return -4;
+    auto go = [&](auto kernel) {
+      return launch_pdl_cluster(kernel, dim3((unsigned)(w_row_tiles * f.splits)), dim3(kF4Threads),
+                                (size_t)(kFewHeader + body), stream, (unsigned)f.splits, tw, tx, tsw, tsx, f);
+    };
+    const cudaError_t e = mx ? (sfb == 1 ? go(fp4_few_kernel<true, 1>) : go(fp4_few_kernel<true, 2>))
+                             : (sfb == 1 ? go(fp4_few_kernel<false, 1>) : go(fp4_few_kernel<false, 2>));
+    return e == cudaSuccess ? 0 : -5;
+  }
+
   Fp4GemmArgs a;
   memset(&a, 0, sizeof(a));
   a.N = N;
   a.M = (int)M;
-  a.kblocks = (K + kF4StepCols - 1) / kF4StepCols;
+  a.kblocks = kblocks;
   const char* forced = getenv("F4_PAIR");
   const bool pair = forced != nullptr ? forced[0] == '1' : tiles != nullptr ? max_tiles > 4 * groups : M > 128;
   a.n_tiles = (N + (pair ? 255 : 127)) / (pair ? 256 : 128);
@@ -541,11 +893,10 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   if (getenv("F4_BN") && M > 256) a.bn = atoi(getenv("F4_BN"));
   a.m_tiles = (int)((M + a.bn - 1) / a.bn);
   a.sfb_tiles = a.bn > 128 ? 2 : 1;
-  const int step_tiles = mx ? 2 : 4;
   a.b_bytes = (uint32_t)(pair ? a.bn / 2 : a.bn) * 128;
   a.sfa_bytes = (uint32_t)step_tiles * kFp4ScaleTile;
   a.sfb_bytes = a.sfa_bytes * (uint32_t)a.sfb_tiles;
-  a.w_row_tiles = (N + 127) / 128;
+  a.w_row_tiles = w_row_tiles;
   a.act = gate != 0 ? gate : act;
   a.has_gate = gate != 0;
   a.gate.limit = gate_limit;
@@ -567,27 +918,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   const long long total = (long long)(tiles != nullptr ? max_tiles : a.m_tiles) * a.n_tiles;
   if (total > 0x7fffffff) return -6;
 
-  const int k_tiles = fp4_k_tiles(K, mx);
-  const long long x_row_tiles = tiles != nullptr ? max_tiles : (M + 127) / 128;
-  CUtensorMap tw, tx, tsw, tsx;
-  {
-    const uint64_t dims[3] = {(uint64_t)K / 2, (uint64_t)N, (uint64_t)groups};
-    const uint64_t strides[2] = {(uint64_t)ldw, (uint64_t)(groups > 1 ? w_gstride : ldw)};
-    const uint32_t box[3] = {128, 128, 1};
-    if (make_tmap_nd(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, dims, strides, box) != 0) return -4;
-  }
-  if (make_tmap_2d(&tx, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K / 2, (uint64_t)ldx,
-                   (uint32_t)(pair ? a.bn / 2 : a.bn), 128) != 0)
-    return -4;
-  auto scales = [&](CUtensorMap* map, const void* base, uint64_t row_tiles, uint32_t box_tiles) {
-    const uint64_t dims[3] = {kFp4ScaleTile / 4, (uint64_t)k_tiles, row_tiles};
-    const uint64_t strides[2] = {kFp4ScaleTile, (uint64_t)k_tiles * kFp4ScaleTile};
-    const uint32_t box[3] = {kFp4ScaleTile / 4, (uint32_t)step_tiles, box_tiles};
-    return make_tmap_nd(map, base, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
-  };
-  if (scales(&tsw, sw, (uint64_t)groups * a.w_row_tiles, 1) != 0 ||
-      scales(&tsx, sx, (uint64_t)x_row_tiles, (uint32_t)a.sfb_tiles) != 0)
-    return -4;
+  if (!make_maps(pair ? a.bn / 2 : a.bn, a.sfb_tiles)) return -4;
   const size_t smem = (size_t)(a.stages * stage + header);
   const long long most = pair ? sms / 2 : sms;
   const dim3 grid((unsigned)((total < most ? total : most) * (pair ? 2 : 1)));
