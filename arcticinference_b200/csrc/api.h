@@ -369,7 +369,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
                      long long w_gstride, const void* sw, const void* gw, void* out, long long ldo, long long M,
                      int N, int K, int groups, int fmt, const void* bias, const void* residual, long long ldr, int act,
                      int gate, float gate_limit, float gate_alpha, const void* tiles, const void* num_tiles,
-                     int max_tiles, int* status, cudaStream_t stream);
+                     int max_tiles, int even, int* status, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

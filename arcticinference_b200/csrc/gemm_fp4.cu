@@ -42,6 +42,7 @@ struct Fp4GemmArgs {
   uint32_t b_bytes, sfa_bytes, sfb_bytes;
   int sfb_tiles;           // row tiles that the scales of a tile's tokens lie in
   int w_row_tiles;         // row tiles of scales per matrix
+  int list_tiles;          // tiles of the list that are taken together: two where groups have an even number
   int act, has_gate;
   GateParams gate;
   const int4* tiles;
@@ -67,11 +68,12 @@ __device__ __forceinline__ F4Work f4_work(const Fp4GemmArgs& p, int w) {
   F4Work r;
   if (p.tiles != nullptr) {
     r.nt = w % p.n_tiles;
-    const int mt = w / p.n_tiles;
+    const int mt = w / p.n_tiles * p.list_tiles;
     const int4 t = p.tiles[mt];
     r.group = t.x;
     r.row0 = t.y;
     r.nrows = t.z;
+    if (p.list_tiles == 2) r.nrows += p.tiles[mt + 1].z;
     r.slot = mt;
     r.shift = 0;
     return r;
@@ -280,7 +282,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();   // (tensor memory is owned)
   pdl_wait();
-  const int total_work = (p.tiles != nullptr ? *p.num_tiles : p.m_tiles) * p.n_tiles;
+  const int total_work = (p.tiles != nullptr ? *p.num_tiles / p.list_tiles : p.m_tiles) * p.n_tiles;
   const int first_work = (int)blockIdx.x / kCtas, work_step = (int)gridDim.x / kCtas;
 
   if (warp == 0) {
@@ -773,12 +775,13 @@ extern "C" {
 // gw fp32 [groups][N] or null; out bf16. K a multiple of 32, N of 8 (of 32 with a gate), strides of codes multiples of
 // 16 bytes, ldo and ldr of 8 elements. fmt: 0 nvfp4, 1 mxfp4. act: 0, 1 (GELU); gate: 0, 1 (silu), 2 (gelu_tanh), 3
 // (clamped swish): rows of w alternate 16 gate and 16 up rows and out has N / 2 columns. With `tiles` (int32 x 4:
-// group, first row, rows; *num_tiles of them, at most max_tiles) row tile i's scales are sx's i-th row tile.
+// group, first row, rows; *num_tiles of them, at most max_tiles) row tile i's scales are sx's i-th row tile; even: every
+// group has an even number of tiles, all but the last two full, of which the last may be empty.
 int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* gx, const void* w, long long ldw,
                      long long w_gstride, const void* sw, const void* gw, void* out, long long ldo, long long M,
                      int N, int K, int groups, int fmt, const void* bias, const void* residual, long long ldr, int act,
                      int gate, float gate_limit, float gate_alpha, const void* tiles, const void* num_tiles,
-                     int max_tiles, int* status, cudaStream_t stream) {
+                     int max_tiles, int even, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || groups <= 0 || (tiles != nullptr && max_tiles <= 0)) return 0;
   auto odd = [](const void* q, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(q) & mask) != 0; };
   if ((K % 32) || (N % 8) || (gate != 0 && N % 32) || gate < 0 || gate > 3 || act < 0 || act > 1 || fmt < 0 || fmt > 1 ||
@@ -889,7 +892,8 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   const bool pair = forced != nullptr ? forced[0] == '1' : tiles != nullptr ? max_tiles > 4 * groups : M > 128;
   a.n_tiles = (N + (pair ? 255 : 127)) / (pair ? 256 : 128);
   const long long split = (M + kF4MaxTokens - 1) / kF4MaxTokens;      // tiles of equal width, in steps of 64
-  a.bn = tiles != nullptr ? 128 : (int)(((M + split - 1) / split + 63) / 64 * 64);
+  a.list_tiles = pair && even ? 2 : 1;
+  a.bn = tiles != nullptr ? 128 * a.list_tiles : (int)(((M + split - 1) / split + 63) / 64 * 64);
   if (getenv("F4_BN") && M > 256) a.bn = atoi(getenv("F4_BN"));
   a.m_tiles = (int)((M + a.bn - 1) / a.bn);
   a.sfb_tiles = a.bn > 128 ? 2 : 1;

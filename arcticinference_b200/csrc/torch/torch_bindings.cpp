@@ -471,7 +471,8 @@ void fp4_dequant(const at::Tensor& q, const at::Tensor& scale, const OptTensor& 
 void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
                  const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt, const OptTensor& bias,
                  const OptTensor& residual, int64_t act, int64_t gate, double limit, double alpha,
-                 const OptTensor& tiles, const OptTensor& num_tiles, at::Tensor& out, const at::Tensor& status) {
+                 const OptTensor& tiles, const OptTensor& num_tiles, bool even, at::Tensor& out,
+                 const at::Tensor& status) {
   const int64_t row_tiles = fp4_tiles(wq, tiles, num_tiles);
   const Fp4Operand w = fp4_operand(wq, ws, wg, fmt, 0, "4-bit weight");
   const c10::cuda::CUDAGuard guard(wq.device());
@@ -536,7 +537,7 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
   check(ab200_linear_fp4(q, ldx, s, g, wq.data_ptr(), wq.stride(-2), wq.dim() == 3 ? wq.stride(0) : 0, ws.data_ptr(),
                          opt_ptr(wg), out.data_ptr(), out.stride(0), M, (int)N, (int)K, (int)w.groups, (int)fmt,
                          opt_ptr(bias), opt_ptr(residual), has(residual) ? residual->stride(0) : 0, (int)act, (int)gate,
-                         (float)limit, (float)alpha, opt_ptr(tiles), opt_ptr(num_tiles), (int)row_tiles,
+                         (float)limit, (float)alpha, opt_ptr(tiles), opt_ptr(num_tiles), (int)row_tiles, even ? 1 : 0,
                          status.data_ptr<int>(), stream),
         "linear_fp4");
 }
@@ -545,7 +546,7 @@ at::Tensor fp4_linear(const OptTensor& x, const OptTensor& xq, const OptTensor& 
                       const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt,
                       const OptTensor& bias, const OptTensor& residual, int64_t act, const at::Tensor& status) {
   at::Tensor out;
-  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, bias, residual, act, 0, 0, 0, {}, {}, out, status);
+  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, bias, residual, act, 0, 0, 0, {}, {}, false, out, status);
   return out;
 }
 
@@ -553,16 +554,17 @@ void fp4_linear_out(const OptTensor& x, const OptTensor& xq, const OptTensor& xs
                     const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt,
                     const OptTensor& bias, const OptTensor& residual, int64_t act, const at::Tensor& status,
                     at::Tensor out) {
-  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, bias, residual, act, 0, 0, 0, {}, {}, out, status);
+  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, bias, residual, act, 0, 0, 0, {}, {}, false, out, status);
 }
 
 at::Tensor fp4_grouped_linear(const OptTensor& x, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
                               const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt,
-                              const at::Tensor& tiles, const at::Tensor& num_tiles, int64_t gate, double limit,
-                              double alpha, const at::Tensor& status) {
+                              const at::Tensor& tiles, const at::Tensor& num_tiles, bool even, int64_t gate,
+                              double limit, double alpha, const at::Tensor& status) {
   TORCH_CHECK_VALUE(wq.dim() == 3, "grouped_linear_fp4: weights [E, N, K]");
   at::Tensor out;
-  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, {}, {}, 0, gate, limit, alpha, tiles, num_tiles, out, status);
+  fp4_product(x, xq, xs, xg, wq, ws, wg, fmt, {}, {}, 0, gate, limit, alpha, tiles, num_tiles, even, out,
+              status);
   return out;
 }
 
@@ -604,7 +606,7 @@ TORCH_LIBRARY(arcticinference_b200, m) {
   m.def("fp4_linear_out(Tensor? x, Tensor? xq, Tensor? xs, Tensor? xg, Tensor wq, Tensor ws, Tensor? wg, int fmt, "
         "Tensor? bias, Tensor? residual, int act, Tensor status, Tensor(a!) out) -> ()");
   m.def("fp4_grouped_linear(Tensor? x, Tensor? xq, Tensor? xs, Tensor? xg, Tensor wq, Tensor ws, Tensor? wg, int fmt, "
-        "Tensor tiles, Tensor num_tiles, int gate, float limit, float alpha, Tensor status) -> Tensor");
+        "Tensor tiles, Tensor num_tiles, bool even, int gate, float limit, float alpha, Tensor status) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(arcticinference_b200, CUDA, m) {

@@ -188,7 +188,7 @@ def grouped_linear_fp4(x, w, routing, act=None) -> torch.Tensor:
     o = _ops()
     launch_counter.add(1 if x is None else 2)
     return o.grouped(x, xq, xs, xg, wq, w.scale, w.row_scale, _FORMATS[w.fmt], routing.tiles, routing.num_tiles,
-                     act.code if act else 0, act.limit if act else 0.0, act.alpha if act else 0.0, o.status(wq.device))
+                     routing.even, act.code if act else 0, act.limit if act else 0.0, act.alpha if act else 0.0, o.status(wq.device))
 
 
 def _grouped_ref(x, w, routing, act):
