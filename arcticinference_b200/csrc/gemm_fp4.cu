@@ -124,26 +124,27 @@ __device__ __forceinline__ uint32_t f4_piece(int token, int piece) {
   return (uint32_t)(token * 64 + ((piece ^ (token >> 1)) & 3) * 16);
 }
 
-// Tokens c0 .. c0 + 31 of a finished tile: lo, hi the warp's first and last 16 features (tmem_ld_frag_x4). Fragments
+// The factor of token c of a tile
+__device__ __forceinline__ float f4_token(const float* x_scale, int row0, int c, int nrows) {
+  return x_scale == nullptr ? 1.f : c < nrows ? x_scale[row0 + c] : 0.f;
+}
+
+// Tokens c0 .. c0 + 31 of a finished tile: lo, hi the warp's first and last 16 features (tmem_ld_frag_x4), gx the factor
+// of token c0 + lane. Fragments
 // are transposed through the staging tile, so that a store has 64 consecutive bytes of eight tokens. Moving them by
 // shuffles, four by four, cost three times the shared-memory cycles, which the products are short of.
 __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t (&lo)[16], const uint32_t (&hi)[16],
                                            uint8_t* stage, int c0, int row0, int nrows, int feature0,
-                                           const F4Features& ft, int lane) {
+                                           const F4Features& ft, float gx, int lane) {
   const uint32_t at = smem_u32(stage);
   float2 g[4];
+  float* cols = reinterpret_cast<float*>(stage);
   __syncwarp();   // (the tile's last readers are done)
-  if (p.x_scale != nullptr) {
-    float* cols = reinterpret_cast<float*>(stage);
-    cols[lane] = c0 + lane < nrows ? p.x_scale[row0 + c0 + lane] : 0.f;
-    __syncwarp();
+  cols[lane] = gx;
+  __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = *reinterpret_cast<const float2*>(cols + 8 * j + 2 * (lane & 3));
-    __syncwarp();
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = make_float2(1.f, 1.f);
-  }
+  for (int j = 0; j < 4; ++j) g[j] = *reinterpret_cast<const float2*>(cols + 8 * j + 2 * (lane & 3));
+  __syncwarp();
   const uint32_t frag = at + f4_piece(lane & 7, lane >> 3);   // + 512 per eight tokens
   if (p.has_gate) {
     // 16 gate rows, then the 16 up rows they belong to
@@ -284,6 +285,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   pdl_wait();
   const int total_work = (p.tiles != nullptr ? *p.num_tiles / p.list_tiles : p.m_tiles) * p.n_tiles;
   const int first_work = (int)blockIdx.x / kCtas, work_step = (int)gridDim.x / kCtas;
+  auto work = [&](int w) {
+    F4Work none = {};
+    return w < total_work ? f4_work(p, w) : none;
+  };
 
   if (warp == 0) {
     // ------------------------------ TMA producer ------------------------------
@@ -291,11 +296,14 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      F4Work t = work(first_work);
       for (int w = first_work; w < total_work && ok; w += work_step) {
-        const F4Work t = f4_work(p, w);
-        if (t.nrows <= 0) continue;
-        const int slice = kCtas * t.nt + rank;       // 128 features
-        const int row = t.row0 + rank * (f4_width(t.nrows) / 2);
+        const F4Work after = work(w + work_step);     // (a list's next entry is on its way meanwhile)
+        const F4Work now = t;
+        t = after;
+        if (now.nrows <= 0) continue;
+        const int slice = kCtas * now.nt + rank;       // 128 features
+        const int row = now.row0 + rank * (f4_width(now.nrows) / 2);
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 1500 + stage, kb)) {
             ok = false;
@@ -307,15 +315,15 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           const uint32_t dst = smem_base + (uint32_t)stage * stage_bytes;
           const uint32_t sfa = dst + kF4ABytes + p.b_bytes;
           if (PAIR) {
-            tma_load_3d_pair(dst, &tmap_w, full, kb * 128, slice * 128, t.group);
+            tma_load_3d_pair(dst, &tmap_w, full, kb * 128, slice * 128, now.group);
             tma_load_2d_pair(dst + kF4ABytes, &tmap_x, full, kb * 128, row);
-            tma_load_3d_pair(sfa, &tmap_sw, full, 0, kb * kTiles, t.group * p.w_row_tiles + slice);
-            tma_load_3d_pair(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, t.slot);
+            tma_load_3d_pair(sfa, &tmap_sw, full, 0, kb * kTiles, now.group * p.w_row_tiles + slice);
+            tma_load_3d_pair(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, now.slot);
           } else {
-            tma_load_3d(dst, &tmap_w, full, kb * 128, slice * 128, t.group);
+            tma_load_3d(dst, &tmap_w, full, kb * 128, slice * 128, now.group);
             tma_load_2d(dst + kF4ABytes, &tmap_x, full, kb * 128, row);
-            tma_load_3d(sfa, &tmap_sw, full, 0, kb * kTiles, t.group * p.w_row_tiles + slice);
-            tma_load_3d(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, t.slot);
+            tma_load_3d(sfa, &tmap_sw, full, 0, kb * kTiles, now.group * p.w_row_tiles + slice);
+            tma_load_3d(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, now.slot);
           }
           if (++stage == p.stages) {
             stage = 0;
@@ -346,8 +354,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       uint32_t set = 0;
       int steps = 0;
       bool ok = true;
+      F4Work coming = work(first_work);
       for (int w = first_work; w < total_work && ok; w += work_step) {
-        const F4Work t = f4_work(p, w);
+        const F4Work t = coming;
+        coming = work(w + work_step);
         if (t.nrows <= 0) continue;
         if (!__all_sync(0xffffffffu, mbar_wait(side_bar(acc), side_phase ^ 1u, abort_flag, p.status, 1600 + acc, w)))
           break;
@@ -433,20 +443,39 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     };
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int w = first_work; w < total_work; w += work_step) {
-      const F4Work t = f4_work(p, w);
-      if (t.nrows <= 0) continue;
-      const int feature0 = (kCtas * t.nt + rank) * 128 + quad * 32;
+    // A tile's factors (and a list's entries) are requested a tile ahead: one after the other they cost a short K more
+    // than its products.
+    struct Factors {
       F4Features ft;
+      float gx[4];
+    };
+    auto fetch = [&](const F4Work& t) {
+      Factors r;
+      const int feature0 = (kCtas * t.nt + rank) * 128 + quad * 32;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int f = min(feature0 + 8 * i + (lane >> 2), p.N - 1);
-        ft.h[i] = p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f;
-        ft.bias[i] = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
+        r.ft.h[i] = p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f;
+        r.ft.bias[i] = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
+        r.gx[i] = f4_token(p.x_scale, t.row0, 32 * half + 64 * i + lane, t.nrows);
       }
+      return r;
+    };
+    F4Work coming = work(first_work);
+    Factors coming_factors = fetch(coming);
+    for (int w = first_work; w < total_work; w += work_step) {
+      const F4Work t = coming;
+      const Factors fc = coming_factors;
+      coming = work(w + work_step);
+      if (t.nrows <= 0) {
+        coming_factors = fetch(coming);
+        continue;
+      }
+      const int feature0 = (kCtas * t.nt + rank) * 128 + quad * 32;
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 1700 + acc, w)))
         break;
       tc_fence_after();
+      coming_factors = fetch(coming);
       const uint32_t t_addr = tmem_base + f4_accumulator(acc, t.nrows) + ((uint32_t)(quad * 32) << 16);
       // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and both
       // handed back as soon as they are in registers.
@@ -469,8 +498,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         for (int i = 0; i < 4; ++i)
           if (i < 2 ? any0 : any1) tmem_ld_wait_dep(r[i]);
         hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
-        if (any0) f4_store32(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, ft, lane);
-        if (any1) f4_store32(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, ft, lane);
+        const bool upper = c0 >= 128;
+        if (any0) f4_store32(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[2] : fc.gx[0], lane);
+        if (any1)
+          f4_store32(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[3] : fc.gx[1], lane);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
@@ -670,17 +701,20 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         ft.h[i] = p.w_scale != nullptr ? p.w_scale[f] : 1.f;
         ft.bias[i] = p.bias != nullptr ? __bfloat162float(p.bias[f]) : 0.f;
       }
+      float gx = f4_token(p.x_scale, 0, 32 * half + lane, p.M);
       ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.status, 1900, n));
       tc_fence_after();
       if (ok && feature0 < p.N)
         for (int c0 = 32 * half; c0 < p.M; c0 += 64) {
+          const float next = f4_token(p.x_scale, 0, c0 + 64 + lane, p.M);
           uint32_t lo[16], hi[16];
           __syncwarp();
           tmem_ld_frag_x4(t_addr + (uint32_t)c0, lo);
           tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), hi);
           tmem_ld_wait_dep(lo);
           tmem_ld_wait_dep(hi);
-          f4_store32(g, lo, hi, ring + (warp - 2) * kF4StoreBytes, c0, 0, p.M, feature0, ft, lane);
+          f4_store32(g, lo, hi, ring + (warp - 2) * kF4StoreBytes, c0, 0, p.M, feature0, ft, gx, lane);
+          gx = next;
         }
     }
   } else {
