@@ -43,7 +43,7 @@ struct Fp4GemmArgs {
   int sfb_tiles;           // row tiles that the scales of a tile's tokens lie in
   int w_row_tiles;         // row tiles of scales per matrix
   int list_tiles;          // tiles of the list that are taken together: two where groups have an even number
-  int act, has_gate;
+  int act;
   GateParams gate;
   const int4* tiles;
   const int* num_tiles;
@@ -129,10 +129,15 @@ __device__ __forceinline__ float f4_token(const float* x_scale, int row0, int c,
   return x_scale == nullptr ? 1.f : c < nrows ? x_scale[row0 + c] : 0.f;
 }
 
+// What an epilogue does, known when it is compiled: the code of all options together does not stay in the instruction
+// cache (a tile of 128 x 256 took 6200 cycles to store, more than the products of a K of 1408).
+enum F4Epilogue : int { kF4Plain = 0, kF4Any = 1, kF4Gate = 2 };   // factors and bias; GELU and residual too; gate / up
+
 // Tokens c0 .. c0 + 31 of a finished tile: lo, hi the warp's first and last 16 features (tmem_ld_frag_x4), gx the factor
 // of token c0 + lane. Fragments
 // are transposed through the staging tile, so that a store has 64 consecutive bytes of eight tokens. Moving them by
 // shuffles, four by four, cost three times the shared-memory cycles, which the products are short of.
+template <int EPI>
 __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t (&lo)[16], const uint32_t (&hi)[16],
                                            uint8_t* stage, int c0, int row0, int nrows, int feature0,
                                            const F4Features& ft, float gx, int lane) {
@@ -146,7 +151,7 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
   for (int j = 0; j < 4; ++j) g[j] = *reinterpret_cast<const float2*>(cols + 8 * j + 2 * (lane & 3));
   __syncwarp();
   const uint32_t frag = at + f4_piece(lane & 7, lane >> 3);   // + 512 per eight tokens
-  if (p.has_gate) {
+  if (EPI == kF4Gate) {
     // 16 gate rows, then the 16 up rows they belong to
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -172,7 +177,7 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
     return;
   }
   const int f = feature0 + 8 * (lane & 3);
-  if (p.residual != nullptr) {
+  if (EPI == kF4Any && p.residual != nullptr) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 8 * i + (lane >> 2);
@@ -192,11 +197,11 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
       v[2 * i] = __uint_as_float(r[0]) * (g[j].x * ft.h[i]) + ft.bias[i];
       v[2 * i + 1] = __uint_as_float(r[1]) * (g[j].y * ft.h[i]) + ft.bias[i];
     }
-    if (p.act == 1) {
+    if (EPI == kF4Any && p.act == 1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = gelu_exact(v[i]);
     }
-    if (p.residual != nullptr) {
+    if (EPI == kF4Any && p.residual != nullptr) {
       uint32_t r[4];
       ldmatrix_t4(frag + 512u * j, r);
 #pragma unroll
@@ -219,7 +224,7 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
   }
 }
 
-template <bool MX, bool PAIR, int SFB>
+template <bool MX, bool PAIR, int SFB, int EPI>
 __global__ void __launch_bounds__(kF4Threads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                 const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
@@ -499,9 +504,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           if (i < 2 ? any0 : any1) tmem_ld_wait_dep(r[i]);
         hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
         const bool upper = c0 >= 128;
-        if (any0) f4_store32(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[2] : fc.gx[0], lane);
+        if (any0) f4_store32<EPI>(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[2] : fc.gx[0], lane);
         if (any1)
-          f4_store32(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[3] : fc.gx[1], lane);
+          f4_store32<EPI>(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[3] : fc.gx[1], lane);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
@@ -555,7 +560,7 @@ __device__ __forceinline__ void st_cluster_v2(uint32_t addr, uint32_t a, uint32_
   asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
 
-template <bool MX, int SFB>
+template <bool MX, int SFB, int EPI>
 __global__ void __launch_bounds__(kF4Threads, SFB == 1 ? 2 : 1)
 fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
@@ -713,7 +718,7 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
           tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), hi);
           tmem_ld_wait_dep(lo);
           tmem_ld_wait_dep(hi);
-          f4_store32(g, lo, hi, ring + (warp - 2) * kF4StoreBytes, c0, 0, p.M, feature0, ft, gx, lane);
+          f4_store32<EPI>(g, lo, hi, ring + (warp - 2) * kF4StoreBytes, c0, 0, p.M, feature0, ft, gx, lane);
           gx = next;
         }
     }
@@ -762,7 +767,7 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         const float* at = reinterpret_cast<const float*>(ring) + (size_t)(8 * part) * pitch + m;
         const float gx = p.x_scale != nullptr ? p.x_scale[m] : 1.f;
         uint4 rq = make_uint4(0, 0, 0, 0);
-        if (p.residual != nullptr) rq = *reinterpret_cast<const uint4*>(p.residual + (long long)m * p.ldr + f);
+        if (EPI == kF4Any && p.residual != nullptr) rq = *reinterpret_cast<const uint4*>(p.residual + (long long)m * p.ldr + f);
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int src = 0; src < p.splits; ++src) {
           const float* a = at + (size_t)src * (source_bytes / 4);
@@ -774,9 +779,9 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         for (int e = 0; e < 8; ++e) {
           const float h = p.w_scale != nullptr ? p.w_scale[f + e] : 1.f;
           v[e] = v[e] * (gx * h) + (p.bias != nullptr ? __bfloat162float(p.bias[f + e]) : 0.f);
-          if (p.act == 1) v[e] = gelu_exact(v[e]);
+          if (EPI == kF4Any && p.act == 1) v[e] = gelu_exact(v[e]);
         }
-        if (p.residual != nullptr) {
+        if (EPI == kF4Any && p.residual != nullptr) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 t = __bfloat1622float2(rp[e]);
@@ -834,17 +839,24 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
     auto large = [](auto kernel) {
       return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess;
     };
-    if (large(fp4_gemm_kernel<false, false, 1>) || large(fp4_gemm_kernel<true, false, 1>) ||
-        large(fp4_gemm_kernel<false, true, 1>) || large(fp4_gemm_kernel<true, true, 1>) ||
-        large(fp4_gemm_kernel<false, false, 2>) || large(fp4_gemm_kernel<true, false, 2>) ||
-        large(fp4_gemm_kernel<false, true, 2>) || large(fp4_gemm_kernel<true, true, 2>) ||
-        large(fp4_few_kernel<false, 1>) || large(fp4_few_kernel<true, 1>) || large(fp4_few_kernel<false, 2>) ||
-        large(fp4_few_kernel<true, 2>) ||
+    auto both = [&](auto a, auto b) { return large(a) || large(b); };
+    if (both(fp4_gemm_kernel<false, false, 1, kF4Plain>, fp4_gemm_kernel<true, false, 1, kF4Plain>) ||
+        both(fp4_gemm_kernel<false, false, 1, kF4Gate>, fp4_gemm_kernel<true, false, 1, kF4Gate>) ||
+        both(fp4_gemm_kernel<false, true, 1, kF4Plain>, fp4_gemm_kernel<true, true, 1, kF4Plain>) ||
+        both(fp4_gemm_kernel<false, true, 1, kF4Any>, fp4_gemm_kernel<true, true, 1, kF4Any>) ||
+        both(fp4_gemm_kernel<false, true, 2, kF4Plain>, fp4_gemm_kernel<true, true, 2, kF4Plain>) ||
+        both(fp4_gemm_kernel<false, true, 2, kF4Any>, fp4_gemm_kernel<true, true, 2, kF4Any>) ||
+        both(fp4_gemm_kernel<false, true, 2, kF4Gate>, fp4_gemm_kernel<true, true, 2, kF4Gate>) ||
+        both(fp4_few_kernel<false, 1, kF4Plain>, fp4_few_kernel<true, 1, kF4Plain>) ||
+        both(fp4_few_kernel<false, 1, kF4Any>, fp4_few_kernel<true, 1, kF4Any>) ||
+        both(fp4_few_kernel<false, 2, kF4Plain>, fp4_few_kernel<true, 2, kF4Plain>) ||
+        both(fp4_few_kernel<false, 2, kF4Any>, fp4_few_kernel<true, 2, kF4Any>) ||
         cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return -3;
     attr_set[dev] = true;
   }
   const int sms = sm_count[dev];
+  const bool plain = act == 0 && residual == nullptr;
   const int step_tiles = mx ? 2 : 4, kblocks = (K + kF4StepCols - 1) / kF4StepCols;
   const int w_row_tiles = (N + 127) / 128, k_tiles = fp4_k_tiles(K, mx);
   CUtensorMap tw, tx, tsw, tsx;
@@ -867,7 +879,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
            scales(&tsx, sx, (uint64_t)(tiles != nullptr ? max_tiles : (M + 127) / 128), (uint32_t)sfb_tiles) == 0;
   };
 
-  if (tiles == nullptr && M <= (getenv("F4_FEW") ? atoi(getenv("F4_FEW")) : 256)) {
+  if (tiles == nullptr && M <= kF4MaxTokens) {
     Fp4FewArgs f;
     memset(&f, 0, sizeof(f));
     f.N = N;
@@ -912,8 +924,12 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
       return launch_pdl_cluster(kernel, dim3((unsigned)(w_row_tiles * f.splits)), dim3(kF4Threads),
                                 (size_t)(kFewHeader + body), stream, (unsigned)f.splits, tw, tx, tsw, tsx, f);
     };
-    const cudaError_t e = mx ? (sfb == 1 ? go(fp4_few_kernel<true, 1>) : go(fp4_few_kernel<true, 2>))
-                             : (sfb == 1 ? go(fp4_few_kernel<false, 1>) : go(fp4_few_kernel<false, 2>));
+    auto by_format = [&](auto nv, auto mxf) { return mx ? go(mxf) : go(nv); };
+    const cudaError_t e =
+        sfb == 1 ? (plain ? by_format(fp4_few_kernel<false, 1, kF4Plain>, fp4_few_kernel<true, 1, kF4Plain>)
+                          : by_format(fp4_few_kernel<false, 1, kF4Any>, fp4_few_kernel<true, 1, kF4Any>))
+                 : (plain ? by_format(fp4_few_kernel<false, 2, kF4Plain>, fp4_few_kernel<true, 2, kF4Plain>)
+                          : by_format(fp4_few_kernel<false, 2, kF4Any>, fp4_few_kernel<true, 2, kF4Any>));
     return e == cudaSuccess ? 0 : -5;
   }
 
@@ -922,11 +938,11 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   a.N = N;
   a.M = (int)M;
   a.kblocks = kblocks;
-  const char* forced = getenv("F4_PAIR");
-  const bool pair = forced != nullptr ? forced[0] == '1' : tiles != nullptr ? max_tiles > 4 * groups : M > 128;
+  // Lists whose groups have an even number of tiles have many rows per group: pairs of CTAs on two tiles at a time.
+  const bool pair = tiles == nullptr || even != 0;
   a.n_tiles = (N + (pair ? 255 : 127)) / (pair ? 256 : 128);
   const long long split = (M + kF4MaxTokens - 1) / kF4MaxTokens;      // tiles of equal width, in steps of 64
-  a.list_tiles = pair && even ? 2 : 1;
+  a.list_tiles = even != 0 ? 2 : 1;
   a.bn = tiles != nullptr ? 128 * a.list_tiles : (int)(((M + split - 1) / split + 63) / 64 * 64);
   if (getenv("F4_BN") && M > 256) a.bn = atoi(getenv("F4_BN"));
   a.m_tiles = (int)((M + a.bn - 1) / a.bn);
@@ -936,7 +952,6 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   a.sfb_bytes = a.sfa_bytes * (uint32_t)a.sfb_tiles;
   a.w_row_tiles = w_row_tiles;
   a.act = gate != 0 ? gate : act;
-  a.has_gate = gate != 0;
   a.gate.limit = gate_limit;
   a.gate.alpha = gate_alpha;
   a.tiles = reinterpret_cast<const int4*>(tiles);
@@ -963,12 +978,19 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   auto go = [&](auto kernel) {
     return launch_pdl_cluster(kernel, grid, dim3(kF4Threads), smem, stream, pair ? 2u : 1u, tw, tx, tsw, tsx, a);
   };
-  auto wide = [&](auto one, auto two) { return a.sfb_tiles == 1 ? go(one) : go(two); };
-  const cudaError_t e =
-      mx ? (pair ? wide(fp4_gemm_kernel<true, true, 1>, fp4_gemm_kernel<true, true, 2>)
-                 : wide(fp4_gemm_kernel<true, false, 1>, fp4_gemm_kernel<true, false, 2>))
-         : (pair ? wide(fp4_gemm_kernel<false, true, 1>, fp4_gemm_kernel<false, true, 2>)
-                 : wide(fp4_gemm_kernel<false, false, 1>, fp4_gemm_kernel<false, false, 2>));
+  auto by_format = [&](auto nv, auto mxf) { return mx ? go(mxf) : go(nv); };
+  cudaError_t e;
+  if (!pair)
+    e = gate != 0 ? by_format(fp4_gemm_kernel<false, false, 1, kF4Gate>, fp4_gemm_kernel<true, false, 1, kF4Gate>)
+                  : by_format(fp4_gemm_kernel<false, false, 1, kF4Plain>, fp4_gemm_kernel<true, false, 1, kF4Plain>);
+  else if (a.sfb_tiles == 1)
+    e = plain ? by_format(fp4_gemm_kernel<false, true, 1, kF4Plain>, fp4_gemm_kernel<true, true, 1, kF4Plain>)
+              : by_format(fp4_gemm_kernel<false, true, 1, kF4Any>, fp4_gemm_kernel<true, true, 1, kF4Any>);
+  else if (gate != 0)
+    e = by_format(fp4_gemm_kernel<false, true, 2, kF4Gate>, fp4_gemm_kernel<true, true, 2, kF4Gate>);
+  else
+    e = plain ? by_format(fp4_gemm_kernel<false, true, 2, kF4Plain>, fp4_gemm_kernel<true, true, 2, kF4Plain>)
+              : by_format(fp4_gemm_kernel<false, true, 2, kF4Any>, fp4_gemm_kernel<true, true, 2, kF4Any>);
   return e == cudaSuccess ? 0 : -5;
 }
 
