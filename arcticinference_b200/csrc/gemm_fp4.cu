@@ -101,14 +101,15 @@ __device__ __forceinline__ uint32_t f4_accumulator(int acc, int nrows) {
 
 __device__ __forceinline__ float gelu_exact(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752f)); }
 
-__device__ __forceinline__ float f4_gated(int act, const GateParams& p, float g, float u) {
+template <int ACT>
+__device__ __forceinline__ float f4_gated(const GateParams& p, float g, float u) {
   float t;   // g * sigmoid(t)
-  if (act == kActClampedSwish) {
+  if (ACT == kActClampedSwish) {
     g = fminf(g, p.limit);
     u = fminf(fmaxf(u, -p.limit), p.limit) + 1.f;
     t = p.alpha * g;
-  } else {
-    t = act == kActSilu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+  } else {   // gelu_tanh(z) = z * sigmoid(2 sqrt(2/pi) (...))
+    t = ACT == kActSilu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
   }
   return __fdividef(g, 1.f + __expf(-t)) * u;
 }
@@ -127,6 +128,26 @@ __device__ __forceinline__ uint32_t f4_piece(int token, int piece) {
 // The factor of token c of a tile
 __device__ __forceinline__ float f4_token(const float* x_scale, int row0, int c, int nrows) {
   return x_scale == nullptr ? 1.f : c < nrows ? x_scale[row0 + c] : 0.f;
+}
+
+// 16 gate rows (lo) and the 16 up rows they belong to (hi), joined into the staging tile
+template <int ACT>
+__device__ __forceinline__ void f4_join(const Fp4GemmArgs& p, const uint32_t (&lo)[16], const uint32_t (&hi)[16],
+                                        const float2 (&g)[4], const F4Features& ft, uint32_t frag, int c0, int nrows) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (c0 + 8 * j >= nrows) break;
+    uint32_t q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float a = f4_gated<ACT>(p.gate, __uint_as_float(lo[4 * j + 2 * i]) * (g[j].x * ft.h[i]),
+                                    __uint_as_float(hi[4 * j + 2 * i]) * (g[j].x * ft.h[2 + i]));
+      const float b = f4_gated<ACT>(p.gate, __uint_as_float(lo[4 * j + 2 * i + 1]) * (g[j].y * ft.h[i]),
+                                    __uint_as_float(hi[4 * j + 2 * i + 1]) * (g[j].y * ft.h[2 + i]));
+      q[i] = pack_bf16x2(a, b);
+    }
+    stmatrix_t2(frag + 512u * j, q[0], q[1]);
+  }
 }
 
 // What an epilogue does, known when it is compiled: the code of all options together does not stay in the instruction
@@ -152,20 +173,9 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
   __syncwarp();
   const uint32_t frag = at + f4_piece(lane & 7, lane >> 3);   // + 512 per eight tokens
   if (EPI == kF4Gate) {
-    // 16 gate rows, then the 16 up rows they belong to
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t q[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float a = f4_gated(p.act, p.gate, __uint_as_float(lo[4 * j + 2 * i]) * (g[j].x * ft.h[i]),
-                                 __uint_as_float(hi[4 * j + 2 * i]) * (g[j].x * ft.h[2 + i]));
-        const float b = f4_gated(p.act, p.gate, __uint_as_float(lo[4 * j + 2 * i + 1]) * (g[j].y * ft.h[i]),
-                                 __uint_as_float(hi[4 * j + 2 * i + 1]) * (g[j].y * ft.h[2 + i]));
-        q[i] = pack_bf16x2(a, b);
-      }
-      stmatrix_t2(frag + 512u * j, q[0], q[1]);
-    }
+    if (p.act == kActSilu) f4_join<kActSilu>(p, lo, hi, g, ft, frag, c0, nrows);
+    else if (p.act == kActGeluTanh) f4_join<kActGeluTanh>(p, lo, hi, g, ft, frag, c0, nrows);
+    else f4_join<kActClampedSwish>(p, lo, hi, g, ft, frag, c0, nrows);
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -480,7 +490,6 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 1700 + acc, w)))
         break;
       tc_fence_after();
-      coming_factors = fetch(coming);
       const uint32_t t_addr = tmem_base + f4_accumulator(acc, t.nrows) + ((uint32_t)(quad * 32) << 16);
       // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and both
       // handed back as soon as they are in registers.
@@ -503,6 +512,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         for (int i = 0; i < 4; ++i)
           if (i < 2 ? any0 : any1) tmem_ld_wait_dep(r[i]);
         hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
+        if (part == 0) coming_factors = fetch(coming);
         const bool upper = c0 >= 128;
         if (any0) f4_store32<EPI>(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[2] : fc.gx[0], lane);
         if (any1)
