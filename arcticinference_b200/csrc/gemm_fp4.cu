@@ -11,7 +11,6 @@
 // scales to tensor memory (sets used in turn) and issues the products into one of two accumulators;
 // eight warps drain the other one.
 
-#include <stdlib.h>
 #include <string.h>
 
 #include "api.h"
@@ -33,7 +32,6 @@ constexpr uint32_t kF4ABytes = 128 * 128;
 // Tensor memory: columns 0 - 383 for two accumulators, then sets of scales. An accumulator of more than 128 tokens
 // takes columns 0 - 255 or 128 - 383: the middle ones belong to both, are drained first and handed on at once.
 constexpr uint32_t kF4Middle = 128, kF4ScaleAt = 384;
-constexpr int kF4MaxTokens = 256;
 
 struct Fp4GemmArgs {
   int N, M, kblocks, n_tiles, m_tiles;
@@ -534,14 +532,15 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------
-// Few tokens (at most 256): the weights are streamed once, which bounds it. A CTA has 128 features and, where these
-// tiles are fewer than the SMs, a part of K: the CTAs of a cluster that share a tile exchange their fp32 sums
-// through shared memory, slices of 16 features, and each adds those of its own slices in the order of K and stores
-// them. The weights' first steps are requested into L2 before the wait for the kernel ahead, whose tail (the rows'
+// Few tokens (at most 128): the weights are streamed once, which bounds it. A CTA has 128 features and, where these
+// tiles are fewer than the SMs, a part of K: the CTAs of a cluster that share a tile send each other their fp32 sums,
+// slices of 16 features, and each adds those of its own slices in the order of K and stores them. The sums go into
+// the sender's shared memory first and from there as bulk copies that complete on a barrier of the receiver; stores
+// into another CTA's memory, eight bytes a lane, and a cluster barrier on either side took 5.5 us for 128 tokens. The weights' first steps are requested into L2 before the wait for the kernel ahead, whose tail (the rows'
 // quantisation) they cover: a prefetch changes no value, whoever has written them.
 struct Fp4FewArgs {
   int N, M, kblocks, splits, per_split, stages;
-  uint32_t b_bytes, columns, scale_at;
+  uint32_t b_bytes, columns, scale_at, recv_at;
   int act;
   const float* x_scale;
   const float* w_scale;
@@ -555,10 +554,9 @@ struct Fp4FewArgs {
 
 constexpr int kFewSlice = 16;                    // features of an exchanged slice
 constexpr uint32_t kFewHeader = 1024;            // barriers in front of the stages
-// Tensor memory: the accumulator, then a set of scales per stage, so that a stage's wait covers its set too. A set of
-// its own for every second step only (as in the kernel above) made a step wait for the one before the last: 0.33
-// instead of 0.15 us a step for one token.
-constexpr uint32_t few_scale_set(int sfb) { return 16u + 16u * (uint32_t)sfb; }
+// Tensor memory: the accumulator, then a set of scales per stage, so that a stage's wait covers its set too.
+constexpr uint32_t kFewScaleSet = 32;
+constexpr int kFewTokens = 128;
 
 __device__ __forceinline__ void tma_prefetch_3d(const void* tmap, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
@@ -566,12 +564,20 @@ __device__ __forceinline__ void tma_prefetch_3d(const void* tmap, int c0, int c1
                "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
-__device__ __forceinline__ void st_cluster_v2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+// `bytes` (a multiple of 16) of this CTA's shared memory into another CTA's, completing on a barrier of that CTA
+__device__ __forceinline__ void bulk_to_cta(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "r"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-template <bool MX, int SFB, int EPI>
-__global__ void __launch_bounds__(kF4Threads, SFB == 1 ? 2 : 1)
+template <bool MX, int EPI>
+__global__ void __launch_bounds__(kF4Threads, 2)
 fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
                const Fp4FewArgs p) {
@@ -585,18 +591,22 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
   }
   constexpr int kTiles = MX ? 2 : 4;
   constexpr uint32_t kSfaBytes = kTiles * kFp4ScaleTile;
-  const uint32_t stage_bytes = kF4ABytes + p.b_bytes + kSfaBytes * (1 + SFB);
+  const uint32_t stage_bytes = kF4ABytes + p.b_bytes + 2 * kSfaBytes;
   const uint32_t base = smem_u32(smem);
   const uint32_t stages0 = base + kFewHeader;
   auto full_bar = [&](int s) { return base + 8u * s; };
   auto empty_bar = [&](int s) { return base + 8u * (kF4MaxStages + s); };
   const uint32_t done_bar = base + 8u * (2 * kF4MaxStages);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 8 * (2 * kF4MaxStages + 1));
+  const uint32_t recv_bar = done_bar + 8u;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 8 * (2 * kF4MaxStages + 2));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* ring = smem + kFewHeader;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int tile = (int)blockIdx.x / p.splits, split = (int)blockIdx.x % p.splits;
+  // sums: [slice][16 features][tokens] floats, sent from where the stages were to a place of their own behind them
+  const int pitch = ((p.M + 31) & ~31) + 8, mine = 8 / p.splits;
+  const uint32_t slice_bytes = (uint32_t)(kFewSlice * pitch) * 4u, source_bytes = slice_bytes * (uint32_t)mine;
   const int k0 = split * p.per_split, n = min(p.per_split, p.kblocks - k0);
 
   if (threadIdx.x == 0) {
@@ -605,8 +615,10 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(done_bar, 1);
+    mbar_init(recv_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
+    if (p.splits > 1) mbar_arrive_expect_tx(recv_bar, (uint32_t)(p.splits - 1) * source_bytes);
     const int ahead = min(n, 2 * p.stages);
     for (int i = 0; i < ahead; ++i) {
       tma_prefetch_3d(&tmap_w, (k0 + i) * 128, tile * 128, 0);
@@ -622,6 +634,7 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();   // (tensor memory is owned)
+  if (p.splits > 1) cluster_arrive();   // (this CTA's receiving barrier is ready)
   pdl_wait();
   bool ok = true;
 
@@ -669,21 +682,18 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
       const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
       const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
       const uint64_t sb_desc = sa_desc + (uint64_t)(kSfaBytes / 16);
-      const uint32_t sfa = tm + p.scale_at + (uint32_t)stage * few_scale_set(SFB), sfb = sfa + 16u;
+      const uint32_t sfa = tm + p.scale_at + (uint32_t)stage * kFewScaleSet, sfb = sfa + 16u;
       if (elect_one()) {
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
           tmem_copy_scales<false>(sfa + 4u * j, sa_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
-#pragma unroll
-          for (int q = 0; q < SFB; ++q)
-            tmem_copy_scales<false>(sfb + 4u * (SFB * j + q),
-                                    sb_desc + (uint64_t)((q * kTiles + j) * (kFp4ScaleTile / 16)));
+          tmem_copy_scales<false>(sfb + 4u * j, sb_desc + (uint64_t)(j * (kFp4ScaleTile / 16)));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int j = MX ? k / 2 : k;
           umma_fp4_ss<MX, false>(tm, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
-                                 MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j, sfb + 4u * SFB * j,
+                                 MX && (k & 1) ? idesc_hi : idesc, sfa + 4u * j, sfb + 4u * j,
                                  (i > 0 || k > 0) ? 1u : 0u);
         }
         tc_commit(empty_bar(stage));
@@ -733,65 +743,98 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         }
     }
   } else {
-    // [source][slice of this CTA][16 features][tokens] floats where the stages were
-    const int pitch = ((p.M + 31) & ~31) + 8, mine = 8 / p.splits;
-    const uint32_t slice_bytes = (uint32_t)(kFewSlice * pitch) * 4u, source_bytes = slice_bytes * (uint32_t)mine;
     const uint32_t my = cluster_ctarank();
-    if (warp >= 2) {
-      ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.status, 1900, n));
-      tc_fence_after();
+    // A thread finishes eight features of every `across`-th token; what it needs beside the sums is requested before
+    // they arrive.
+    const int tid = (int)threadIdx.x - 64, across = kF4EpilogueWarps * 32 / (2 * mine);
+    const int part = tid / across, first = tid % across;
+    const int f = tile * 128 + (int)my * mine * kFewSlice + 8 * part;
+    const bool mine_too = warp >= 2 && warp < 2 + kF4EpilogueWarps && f < p.N;
+    float h[8], bias[8], gx = 1.f;
+    uint4 rq = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      h[e] = 1.f;
+      bias[e] = 0.f;
     }
-    __syncthreads();
-    cluster_sync();   // every CTA of the cluster has read its last stage
-    if (warp >= 2 && ok) {
-      for (int c0 = 32 * half; c0 < p.M; c0 += 64) {
-        uint32_t r[2][16];
-        __syncwarp();
-        tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
-        tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
-        tmem_ld_wait_dep(r[0]);
-        tmem_ld_wait_dep(r[1]);
+    if (mine_too) {
+      if (p.w_scale != nullptr) {
+        const float4 a = load4(p.w_scale + f), b = load4(p.w_scale + f + 4);
+        h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
+        h[4] = b.x; h[5] = b.y; h[6] = b.z; h[7] = b.w;
+      }
+      if (p.bias != nullptr) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int slice = 2 * quad + h;
-          const uint32_t to = map_to_cta(stages0 + my * source_bytes + (uint32_t)(slice % mine) * slice_bytes +
-                                             (uint32_t)((lane >> 2) * pitch + c0 + 2 * (lane & 3)) * 4u,
-                                         (uint32_t)(slice / mine));
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (c0 + 8 * j < p.M) {
-              st_cluster_v2(to + 32u * j, r[h][4 * j], r[h][4 * j + 1]);
-              st_cluster_v2(to + 32u * j + 32u * (uint32_t)pitch, r[h][4 * j + 2], r[h][4 * j + 3]);
-            }
-        }
+        for (int e = 0; e < 8; ++e) bias[e] = __bfloat162float(p.bias[f + e]);
+      }
+      if (first < p.M) {
+        gx = f4_token(p.x_scale, 0, first, p.M);
+        if (EPI == kF4Any && p.residual != nullptr)
+          rq = *reinterpret_cast<const uint4*>(p.residual + (long long)first * p.ldr + f);
       }
     }
-    cluster_sync();
-    if (warp >= 2 && ok) {
-      // eight features of a token each
-      const int items = 2 * mine * p.M;
-      for (int it = (int)threadIdx.x - 64; it < items; it += kF4EpilogueWarps * 32) {
-        const int part = it / p.M, m = it - part * p.M;
-        const int f = tile * 128 + (int)my * mine * kFewSlice + 8 * part;
-        if (f >= p.N) continue;
-        const float* at = reinterpret_cast<const float*>(ring) + (size_t)(8 * part) * pitch + m;
-        const float gx = p.x_scale != nullptr ? p.x_scale[m] : 1.f;
-        uint4 rq = make_uint4(0, 0, 0, 0);
-        if (EPI == kF4Any && p.residual != nullptr) rq = *reinterpret_cast<const uint4*>(p.residual + (long long)m * p.ldr + f);
+    if (warp >= 2 && warp < 2 + kF4EpilogueWarps) {
+      ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.status, 1900, n));
+      tc_fence_after();
+      if (ok)
+        for (int c0 = 32 * half; c0 < p.M; c0 += 64) {
+          uint32_t r[2][16];
+          __syncwarp();
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
+          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
+          tmem_ld_wait_dep(r[0]);
+          tmem_ld_wait_dep(r[1]);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float* to = reinterpret_cast<float*>(ring + (uint32_t)(2 * quad + q) * slice_bytes) +
+                        (lane >> 2) * pitch + c0 + 2 * (lane & 3);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              *reinterpret_cast<uint2*>(to + 8 * j) = make_uint2(r[q][4 * j], r[q][4 * j + 1]);
+              *reinterpret_cast<uint2*>(to + 8 * j + 8 * pitch) = make_uint2(r[q][4 * j + 2], r[q][4 * j + 3]);
+            }
+          }
+        }
+      fence_proxy_async_smem();
+    }
+    __syncthreads();
+    cluster_wait();   // every receiver is ready
+    if (warp == 2 && lane < p.splits && lane != (int)my) {
+      const uint32_t place = (uint32_t)((int)my < lane ? (int)my : (int)my - 1) * source_bytes;
+      bulk_to_cta(map_to_cta(base + p.recv_at + place, (uint32_t)lane), stages0 + (uint32_t)lane * source_bytes,
+                  source_bytes, map_to_cta(recv_bar, (uint32_t)lane));
+    }
+    __syncwarp();
+    if (warp >= 2 && warp < 2 + kF4EpilogueWarps)
+      ok = __all_sync(0xffffffffu, mbar_wait(recv_bar, 0, abort_flag, p.status, 1910, n)) && ok;
+    __syncwarp();
+    cluster_arrive();   // (nobody leaves before its sums have been received)
+    if (mine_too && ok) {
+      const float* own = reinterpret_cast<const float*>(ring + my * source_bytes) + (size_t)(8 * part) * pitch;
+      const float* others = reinterpret_cast<const float*>(smem + p.recv_at) + (size_t)(8 * part) * pitch;
+      for (int m = first; m < p.M; m += across) {
+        const int after = m + across;
+        float next_gx = 1.f;
+        uint4 next_rq = make_uint4(0, 0, 0, 0);
+        if (after < p.M) {
+          next_gx = f4_token(p.x_scale, 0, after, p.M);
+          if (EPI == kF4Any && p.residual != nullptr)
+            next_rq = *reinterpret_cast<const uint4*>(p.residual + (long long)after * p.ldr + f);
+        }
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int src = 0; src < p.splits; ++src) {
-          const float* a = at + (size_t)src * (source_bytes / 4);
+          const float* a = (src == (int)my ? own
+                                           : others + (size_t)(src < (int)my ? src : src - 1) * (source_bytes / 4)) + m;
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] += a[e * pitch];
         }
-        const __nv_bfloat162* rp = reinterpret_cast<const __nv_bfloat162*>(&rq);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float h = p.w_scale != nullptr ? p.w_scale[f + e] : 1.f;
-          v[e] = v[e] * (gx * h) + (p.bias != nullptr ? __bfloat162float(p.bias[f + e]) : 0.f);
+          v[e] = v[e] * (gx * h[e]) + bias[e];
           if (EPI == kF4Any && p.act == 1) v[e] = gelu_exact(v[e]);
         }
         if (EPI == kF4Any && p.residual != nullptr) {
+          const __nv_bfloat162* rp = reinterpret_cast<const __nv_bfloat162*>(&rq);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 t = __bfloat1622float2(rp[e]);
@@ -802,8 +845,12 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         *reinterpret_cast<uint4*>(p.out + (long long)m * p.ldo + f) =
             make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                        pack_bf16x2(v[6], v[7]));
+        gx = next_gx;
+        rq = next_rq;
       }
     }
+    __syncwarp();
+    cluster_wait();
   }
   tc_fence_before();
   __syncthreads();
@@ -857,10 +904,8 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
         both(fp4_gemm_kernel<false, true, 2, kF4Plain>, fp4_gemm_kernel<true, true, 2, kF4Plain>) ||
         both(fp4_gemm_kernel<false, true, 2, kF4Any>, fp4_gemm_kernel<true, true, 2, kF4Any>) ||
         both(fp4_gemm_kernel<false, true, 2, kF4Gate>, fp4_gemm_kernel<true, true, 2, kF4Gate>) ||
-        both(fp4_few_kernel<false, 1, kF4Plain>, fp4_few_kernel<true, 1, kF4Plain>) ||
-        both(fp4_few_kernel<false, 1, kF4Any>, fp4_few_kernel<true, 1, kF4Any>) ||
-        both(fp4_few_kernel<false, 2, kF4Plain>, fp4_few_kernel<true, 2, kF4Plain>) ||
-        both(fp4_few_kernel<false, 2, kF4Any>, fp4_few_kernel<true, 2, kF4Any>) ||
+        both(fp4_few_kernel<false, kF4Plain>, fp4_few_kernel<true, kF4Plain>) ||
+        both(fp4_few_kernel<false, kF4Any>, fp4_few_kernel<true, kF4Any>) ||
         cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return -3;
     attr_set[dev] = true;
@@ -889,37 +934,47 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
            scales(&tsx, sx, (uint64_t)(tiles != nullptr ? max_tiles : (M + 127) / 128), (uint32_t)sfb_tiles) == 0;
   };
 
-  if (tiles == nullptr && M <= kF4MaxTokens) {
+  if (tiles == nullptr && M <= kFewTokens) {
     Fp4FewArgs f;
     memset(&f, 0, sizeof(f));
     f.N = N;
     f.M = (int)M;
     f.kblocks = kblocks;
-    const int x_rows = (int)(M + 15) / 16 * 16, sfb = M > 128 ? 2 : 1;
+    const int x_rows = (int)(M + 15) / 16 * 16;
     f.b_bytes = (uint32_t)x_rows * 128;
-    const uint64_t stage = kF4ABytes + f.b_bytes + (uint64_t)step_tiles * kFp4ScaleTile * (1 + sfb);
-    // More tiles than SMs: two CTAs on each, with half of its shared and tensor memory (for up to 128 tokens). Fewer: a
-    // tile's steps are split.
-    const int per_sm = sfb == 1 && w_row_tiles > sms ? 2 : 1;
+    const uint64_t stage = kF4ABytes + f.b_bytes + 2ull * step_tiles * kFp4ScaleTile;
+    // More tiles than SMs: two CTAs on each, with half of its shared and tensor memory. Fewer: a tile's steps are
+    // split.
+    const int per_sm = w_row_tiles > sms ? 2 : 1;
+    // (0.31 us a step; the exchange 1.0 to 2.0 us between two CTAs, 1.8 to 3.7 between four, by the tokens: 4096 x 4096,
+    // 1, 64 and 128 tokens 7.2, 7.5, 8.5 us unsplit, 5.7, 6.5, 7.8 with two parts, 5.2, 6.6, 8.4 with four; eight never paid)
     f.splits = 1;
-    while (f.splits < 8 && w_row_tiles * f.splits * 2 <= sms && kblocks >= 2 * f.splits) f.splits *= 2;
-    if (getenv("F4_SPLITS")) f.splits = atoi(getenv("F4_SPLITS"));
+    double least = 0.31 * kblocks;
+    for (int parts = 2; parts <= 4 && w_row_tiles * parts <= sms; parts *= 2) {
+      const double t = 0.31 * kblocks / parts + (parts == 2 ? 1.0 + 0.008 * (double)M : 1.8 + 0.015 * (double)M);
+      if (t < least) {
+        least = t;
+        f.splits = parts;
+      }
+    }
     f.per_split = (kblocks + f.splits - 1) / f.splits;
     while (f.splits > 1 && f.per_split * (f.splits - 1) >= kblocks) {   // every CTA of a cluster has work
       f.splits /= 2;
       f.per_split = (kblocks + f.splits - 1) / f.splits;
     }
-    const uint64_t exchange =
-        f.splits > 1 ? (uint64_t)8 * kFewSlice * (((M + 31) & ~31ll) + 8) * 4 : kF4EpilogueWarps * kF4StoreBytes;
+    const uint64_t slice = (uint64_t)kFewSlice * (((M + 31) & ~31ll) + 8) * 4;
+    const uint64_t send = f.splits > 1 ? 8 * slice : kF4EpilogueWarps * kF4StoreBytes;
+    const uint64_t receive = f.splits > 1 ? (uint64_t)(f.splits - 1) * (8 / f.splits) * slice : 0;
     f.columns = per_sm == 2 ? 256 : 512;
-    f.scale_at = M <= 64 ? 64 : M <= 128 ? 128 : 256;
-    const int sets = (int)((f.columns - f.scale_at) / few_scale_set(sfb));
-    f.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - kFewHeader) / stage);
+    f.scale_at = M <= 64 ? 64 : 128;
+    const int sets = (int)((f.columns - f.scale_at) / kFewScaleSet);
+    f.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - kFewHeader - receive) / stage);
     if (f.stages > kF4MaxStages) f.stages = kF4MaxStages;
     if (f.stages > sets) f.stages = sets;
     if (f.stages > f.per_split) f.stages = f.per_split;
     uint64_t body = f.stages * stage;
-    if (body < exchange) body = exchange;
+    if (body < send) body = send;
+    f.recv_at = (uint32_t)(kFewHeader + body);
     f.act = act;
     f.x_scale = reinterpret_cast<const float*>(gx);
     f.w_scale = reinterpret_cast<const float*>(gw);
@@ -929,17 +984,14 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
     f.out = reinterpret_cast<bf16*>(out);
     f.ldo = ldo;
     f.status = status;
-    if (!make_maps(x_rows, sfb)) return -4;
+    if (!make_maps(x_rows, 1)) return -4;
     auto go = [&](auto kernel) {
       return launch_pdl_cluster(kernel, dim3((unsigned)(w_row_tiles * f.splits)), dim3(kF4Threads),
-                                (size_t)(kFewHeader + body), stream, (unsigned)f.splits, tw, tx, tsw, tsx, f);
+                                (size_t)(kFewHeader + body + receive), stream, (unsigned)f.splits, tw, tx, tsw, tsx, f);
     };
     auto by_format = [&](auto nv, auto mxf) { return mx ? go(mxf) : go(nv); };
-    const cudaError_t e =
-        sfb == 1 ? (plain ? by_format(fp4_few_kernel<false, 1, kF4Plain>, fp4_few_kernel<true, 1, kF4Plain>)
-                          : by_format(fp4_few_kernel<false, 1, kF4Any>, fp4_few_kernel<true, 1, kF4Any>))
-                 : (plain ? by_format(fp4_few_kernel<false, 2, kF4Plain>, fp4_few_kernel<true, 2, kF4Plain>)
-                          : by_format(fp4_few_kernel<false, 2, kF4Any>, fp4_few_kernel<true, 2, kF4Any>));
+    const cudaError_t e = plain ? by_format(fp4_few_kernel<false, kF4Plain>, fp4_few_kernel<true, kF4Plain>)
+                                : by_format(fp4_few_kernel<false, kF4Any>, fp4_few_kernel<true, kF4Any>);
     return e == cudaSuccess ? 0 : -5;
   }
 
@@ -951,10 +1003,23 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   // Lists whose groups have an even number of tiles have many rows per group: pairs of CTAs on two tiles at a time.
   const bool pair = tiles == nullptr || even != 0;
   a.n_tiles = (N + (pair ? 255 : 127)) / (pair ? 256 : 128);
-  const long long split = (M + kF4MaxTokens - 1) / kF4MaxTokens;      // tiles of equal width, in steps of 64
   a.list_tiles = even != 0 ? 2 : 1;
-  a.bn = tiles != nullptr ? 128 * a.list_tiles : (int)(((M + split - 1) / split + 63) / 64 * 64);
-  if (getenv("F4_BN") && M > 256) a.bn = atoi(getenv("F4_BN"));
+  a.bn = 128 * a.list_tiles;
+  if (tiles == nullptr) {
+    // Width of the token tiles: waves of pairs times what 16 steps of a tile take (measured with N = 28672, M = 1500: 77,
+    // 87, 111 and 206 us for 256, 192, 128 and 64; M = 300, N = 4096: 11.0, 10.5, 9.6, 13.9).
+    const int width[4] = {256, 192, 128, 64};
+    const double us[4] = {7.7, 6.7, 5.9, 5.6};
+    double best = 1e30;
+    for (int i = 0; i < 4; ++i) {
+      const long long items = (M + width[i] - 1) / width[i] * a.n_tiles, pairs = sms / 2;
+      const double t = (double)((items + pairs - 1) / pairs) * us[i];
+      if (t < best) {
+        best = t;
+        a.bn = width[i];
+      }
+    }
+  }
   a.m_tiles = (int)((M + a.bn - 1) / a.bn);
   a.sfb_tiles = a.bn > 128 ? 2 : 1;
   a.b_bytes = (uint32_t)(pair ? a.bn / 2 : a.bn) * 128;

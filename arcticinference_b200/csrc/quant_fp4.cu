@@ -412,6 +412,7 @@ static int launch_quant_fp4(const QuantFp4Args& a, long long M, cudaStream_t str
   const bool many = M >= 148 * 8;
   if (vecs <= 64) return go(quant_fp4_kernel<SRC, MX, 2, true>, (M + 3) / 4, 128);
   if (vecs <= 128 && many) return go(quant_fp4_kernel<SRC, MX, 4, true>, (M + 3) / 4, 128);
+  if (SRC == kFp4Plain && vecs <= 256 && many) return go(quant_fp4_kernel<SRC, MX, 8, true>, (M + 3) / 4, 128);
   int vpt = !many ? 2 : SRC == kFp4Silu ? 4 : 8;
   while (vecs > 512 * vpt) vpt *= 2;
   const int threads = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
