@@ -490,7 +490,7 @@ class ModelConfig:
     hidden_act: str = "silu"
     # weights
     dtype: str = "bfloat16"
-    quantization: Optional[str] = None  # None | "fp8"
+    quantization: Optional[str] = None  # None | "fp8" | "nvfp4" | "mxfp4"
     fp8_block_size: int = 128
     # "channel": a scale per output feature, activations per token; "block": 128 x 128 blocks
     fp8_scheme: str = "channel"
@@ -557,8 +557,14 @@ class ModelConfig:
             raise ValueError("num_attention_heads must be a multiple of num_key_value_heads")
         if self.head_dim not in (64, 128):
             raise ValueError("head_dim must be 64 or 128 (tensor-memory attention tiles)")
-        if self.quantization not in (None, "fp8"):
-            raise ValueError("quantization must be None or 'fp8'")
+        if self.quantization not in (None, "fp8", "nvfp4", "mxfp4"):
+            raise ValueError("quantization must be None, 'fp8', 'nvfp4' or 'mxfp4'")
+        if self.quantization in ("nvfp4", "mxfp4") and (
+                self.hidden_size % 32 or self.intermediate_size % 32 or
+                self.num_attention_heads * self.head_dim % 32 or
+                self.hidden_size > 16384 or self.intermediate_size > 32768):
+            raise NotImplementedError("4-bit linears need widths that are multiples of 32, up to 16384 (hidden) and "
+                                      "32768 (intermediate)")
         if self.fp8_scheme not in ("channel", "block"):
             raise ValueError("fp8_scheme must be 'channel' or 'block'")
         if (self.qk_norm or self.qkv_bias) and self.is_swiftkv:
@@ -1082,6 +1088,9 @@ class EngineConfig:
                              (m.num_attention_heads, ways))
         if m.num_key_value_heads % p.tp and p.tp % m.num_key_value_heads:
             raise ValueError("num_key_value_heads and tensor_parallel_size must divide evenly")
+        if m.quantization in ("nvfp4", "mxfp4") and p.world_size > 1:
+            raise NotImplementedError("quantization=%r on several GPUs: the 4-bit linears have neither shards of K nor "
+                                      "cross-rank signals; use fp8" % m.quantization)
         if m.is_swiftkv and p.pipeline_parallel_size > 1:
             raise ValueError("SwiftKV models do not support pipeline parallelism")
         if m.sliding_window is not None and self.scheduler.max_model_len > m.sliding_window:
@@ -1209,7 +1218,7 @@ class EngineArgs:
         g.add_argument("--tokenizer", type=str, default=None)
         g.add_argument("--served-model-name", type=str, default=None)
         g.add_argument("--dtype", type=str, default="bfloat16")
-        g.add_argument("--quantization", "-q", type=str, default=None, choices=[None, "fp8"])
+        g.add_argument("--quantization", "-q", type=str, default=None, choices=[None, "fp8", "nvfp4", "mxfp4"])
         g.add_argument("--fp8-scheme", type=str, default=None, choices=[None, "channel", "block"],
                        help="fp8 scale layout: one scale per output feature with per-token "
                             "activation scales (default), or 128 x 128 blocks")

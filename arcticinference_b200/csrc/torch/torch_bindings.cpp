@@ -449,8 +449,8 @@ Fp4Operand fp4_operand(const at::Tensor& q, const at::Tensor& scale, const OptTe
   return o;
 }
 
-void fp4_dequant(const at::Tensor& q, const at::Tensor& scale, const OptTensor& row_scale, int64_t fmt,
-                 const OptTensor& tiles, const OptTensor& num_tiles, at::Tensor out) {
+void fp4_dequant_out(const at::Tensor& q, const at::Tensor& scale, const OptTensor& row_scale, int64_t fmt,
+                     const OptTensor& tiles, const OptTensor& num_tiles, at::Tensor out) {
   const int64_t row_tiles = fp4_tiles(q, tiles, num_tiles);
   const Fp4Operand o = fp4_operand(q, scale, row_scale, fmt, row_tiles, "dequant_fp4");
   TORCH_CHECK_VALUE(q.dim() == 2 || q.stride(0) == q.stride(1) * q.size(1), "dequant_fp4: matrices behind one another");
@@ -465,6 +465,16 @@ void fp4_dequant(const at::Tensor& q, const at::Tensor& scale, const OptTensor& 
     check(ab200_dequant_fp4(q.data_ptr(), q.stride(-2), scale.data_ptr(), opt_ptr(row_scale), out.data_ptr(), o.K, R,
                             (int)o.K, (int)o.rows, (int)fmt, opt_ptr(tiles), opt_ptr(num_tiles), stream_of(q)),
           "dequant_fp4");
+}
+
+at::Tensor fp4_dequant(const at::Tensor& q, const at::Tensor& scale, const OptTensor& row_scale, int64_t fmt,
+                       const OptTensor& tiles, const OptTensor& num_tiles) {
+  TORCH_CHECK_VALUE(q.dim() == 2 || q.dim() == 3, "dequant_fp4: codes [.., rows, K / 2]");
+  const auto options = q.options().dtype(at::kBFloat16);
+  at::Tensor out = q.dim() == 2 ? at::empty({q.size(0), 2 * q.size(1)}, options)
+                                : at::empty({q.size(0), q.size(1), 2 * q.size(2)}, options);
+  fp4_dequant_out(q, scale, row_scale, fmt, tiles, num_tiles, out);
+  return out;
 }
 
 // x: bf16 rows, quantised here into scratch, or xq, xs, xg
@@ -599,7 +609,8 @@ TORCH_LIBRARY(arcticinference_b200, m) {
   m.def("fp4_quant(Tensor x, int fmt, Tensor? tiles=None, Tensor? num_tiles=None) -> (Tensor, Tensor, Tensor)");
   m.def("fp4_rmsnorm(Tensor x, Tensor weight, float eps, Tensor(a!)? residual, int fmt) -> (Tensor, Tensor, Tensor)");
   m.def("fp4_silu_mul(Tensor x, int nblk, int fmt) -> (Tensor, Tensor, Tensor)");
-  m.def("fp4_dequant(Tensor q, Tensor scale, Tensor? row_scale, int fmt, Tensor? tiles, Tensor? num_tiles, "
+  m.def("fp4_dequant(Tensor q, Tensor scale, Tensor? row_scale, int fmt, Tensor? tiles, Tensor? num_tiles) -> Tensor");
+  m.def("fp4_dequant_out(Tensor q, Tensor scale, Tensor? row_scale, int fmt, Tensor? tiles, Tensor? num_tiles, "
         "Tensor(a!) out) -> ()");
   m.def("fp4_linear(Tensor? x, Tensor? xq, Tensor? xs, Tensor? xg, Tensor wq, Tensor ws, Tensor? wg, int fmt, "
         "Tensor? bias, Tensor? residual, int act, Tensor status) -> Tensor");
@@ -628,6 +639,7 @@ TORCH_LIBRARY_IMPL(arcticinference_b200, CUDA, m) {
   m.impl("fp4_rmsnorm", &fp4_rmsnorm);
   m.impl("fp4_silu_mul", &fp4_silu_mul);
   m.impl("fp4_dequant", &fp4_dequant);
+  m.impl("fp4_dequant_out", &fp4_dequant_out);
   m.impl("fp4_linear", &fp4_linear);
   m.impl("fp4_linear_out", &fp4_linear_out);
   m.impl("fp4_grouped_linear", &fp4_grouped_linear);

@@ -173,6 +173,9 @@ class ModelRunner:
             self.model.init_random(cfg.seed)
         else:
             self.model.load_weights(cfg.model.name_or_path)
+        if cfg.model.quantization in ("nvfp4", "mxfp4"):
+            from ..models.quant import quantize_model_fp4
+            quantize_model_fp4(self.model, cfg.model.quantization)
         if cfg.model.quantization == "fp8":
             from ..models.quant import quantize_model_fp8
             quantize_model_fp8(self.model, scheme=cfg.model.fp8_scheme)

@@ -30,13 +30,15 @@ def _model_tensors(engine):
         items.extend(prop.weight_slots())
     # an fp8 weight is two tensors (codes, block scales); its bf16 prefill shadow is derived
     # data, dropped while asleep and rebuilt on wake
-    from ..models.quant import Fp8Weight
+    from ..models.quant import Fp4Weight, Fp8Weight
     out = []
     for owner, name in items:
         t = _get(owner, name) if (isinstance(owner, dict) and name in owner) or \
             (not isinstance(owner, dict) and hasattr(owner, name)) else None
         if isinstance(t, Fp8Weight):
             out.extend([(t, "q"), (t, "scale")])
+        elif isinstance(t, Fp4Weight):
+            out.extend([(t, "q"), (t, "scale")] + ([] if t.row_scale is None else [(t, "row_scale")]))
         else:
             out.append((owner, name))
     return out

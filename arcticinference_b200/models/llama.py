@@ -181,8 +181,9 @@ class LlamaModel:
         self.inv_freq = compute_inv_freq(cfg, self.device)
         self.scale = rope_attention_factor(cfg) ** 2 / math.sqrt(self.D)
         self.n_kv_layers = cfg.num_key_value_layers if cfg.is_swiftkv else cfg.num_hidden_layers
-        # fp8 weights with per-token activation scales: the norm and SiLU kernels that feed the
-        # linear layers emit quantised rows directly (set by quantize_model_fp8)
+        # fp8 weights with per-token activation scales (True) or 4-bit weights (their format): the norm and
+        # SiLU kernels that feed the linear layers emit quantised rows directly (set by
+        # quantize_model_fp8 and quantize_model_fp4)
         self.act_quant = False
         # pipeline parallelism (parallel/pipeline.py): this rank keeps the layers
         # [layer_lo, layer_hi) only; embedding on the first stage, norm + LM head on the last

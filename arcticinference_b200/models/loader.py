@@ -309,12 +309,11 @@ class LlamaWeightUpdater:
 
     def _apply_layer(self, l: int, d: dict) -> None:
         from ..server.weight_sync.utils import assign_in_place
-        from .quant import Fp8Weight
         m = self.model
         old = m.layers[l]
         later = m.cfg.is_swiftkv and l >= m.n_kv_layers
         real_wkv = m.wkv_swiftkv
-        if later and isinstance(real_wkv, Fp8Weight):
+        if later and real_wkv is not None and not isinstance(real_wkv, torch.Tensor):
             # pack into a dense staging copy; re-quantised once at the end
             if self._wkv_stage is None:
                 self._wkv_stage = real_wkv.dequantize()

@@ -513,3 +513,24 @@ def quantize_weight_fp4(w: torch.Tensor, fmt: str = "nvfp4") -> Fp4Weight:
         return Fp4Weight(r.q, r.scale, r.row_scale, fmt)
     return Fp4Weight(torch.stack([r.q for r in parts]), torch.stack([r.scale for r in parts]),
                      None if parts[0].row_scale is None else torch.stack([r.row_scale for r in parts]), fmt)
+
+
+def quantize_model_fp4(model, fmt: str = "nvfp4") -> None:
+    """Replace the linear weights of a decoder by 4-bit ones (embeddings, norms and the LM head stay in bf16); their
+    activations are then quantised by the norm and SiLU kernels, or in the linear layer's own call. One GPU."""
+    check_fp4_format(fmt)
+    if int(getattr(model, "n_stored", 1)) != 1:
+        raise NotImplementedError("4-bit weights of a sharded model")
+    for lw in model.layers:
+        if lw is None:
+            continue
+        for name in ("wqkv", "wo", "wgu", "wdown"):
+            w = getattr(lw, name)
+            if isinstance(w, torch.Tensor):
+                setattr(lw, name, quantize_weight_fp4(w, fmt))
+                del w
+    if isinstance(getattr(model, "wkv_swiftkv", None), torch.Tensor):
+        model.wkv_swiftkv = quantize_weight_fp4(model.wkv_swiftkv, fmt)
+    model.act_quant = fmt
+    if torch.cuda.is_available() and model.device.type == "cuda":
+        torch.cuda.empty_cache()

@@ -30,7 +30,8 @@ class _Ops:
         from . import native
         t = build.load_torch_ops()
         self.quant, self.rmsnorm, self.silu_mul = t.fp4_quant.default, t.fp4_rmsnorm.default, t.fp4_silu_mul.default
-        self.dequant, self.linear = t.fp4_dequant.default, t.fp4_linear.default
+        self.dequant, self.dequant_out = t.fp4_dequant.default, t.fp4_dequant_out.default
+        self.linear = t.fp4_linear.default
         self.linear_out, self.grouped = t.fp4_linear_out.default, t.fp4_grouped_linear.default
         self.status, self.rows = native.status_buffer, quant.Fp4Rows._of
 
@@ -61,9 +62,9 @@ def _bf16_matrix(x, what: str) -> None:
 def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", routing=None):
     """bf16 rows [M, K], K a multiple of 32 and at most 32768 -> ``Fp4Rows``. ``routing`` (a ``stream_ops.Routing``): the
     rows are sorted by expert and lie in its tiles; rows that no tile holds are left out."""
-    from ..models import quant
     code = _code(fmt)
     if not x.is_cuda:
+        from ..models import quant
         _bf16_matrix(x, "quant_fp4")
         K = x.shape[1]
         _need(K % 32 == 0 and 0 < K <= 32768, "quant_fp4: K a multiple of 32 up to 32768, got %d", K)
@@ -78,17 +79,18 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", routing=None):
 def dequant_fp4(rows, out: torch.Tensor = None) -> torch.Tensor:
     """The bf16 numbers that ``rows`` (``Fp4Rows`` or ``Fp4Weight``) stand for, each rounded once; exact where the row
     factors are powers of two, as the quantisers' are. With a routing, rows that no tile holds are not written."""
-    from ..models import quant
     if not rows.is_cuda:
+        from ..models import quant
         plain = rows if rows.routing is None else quant.Fp4Rows(rows.q, rows.scale, rows.row_scale, rows.fmt)
         y = quant.dequantize_fp4_ref(plain).to(torch.bfloat16)
         return y if out is None else out.copy_(y)
-    if out is None:
-        out = torch.empty(rows.shape, dtype=torch.bfloat16, device=rows.device)
-    r = rows.routing
-    _ops().dequant(rows.q, rows.scale, rows.row_scale, _FORMATS[rows.fmt], None if r is None else r.tiles,
-                   None if r is None else r.num_tiles, out)
+    r, o = rows.routing, _ops()
+    args = (rows.q, rows.scale, rows.row_scale, _FORMATS[rows.fmt], None if r is None else r.tiles,
+            None if r is None else r.num_tiles)
     launch_counter.add(1)
+    if out is None:
+        return o.dequant(*args)
+    o.dequant_out(*args, out)
     return out
 
 

@@ -105,3 +105,30 @@ def routing_of(counts, device, even=False, slack=3):
     tiles += [(7, 1 << 20, 99, 0)] * slack
     return stream_ops.Routing(None, None, None, 1, len(counts), torch.tensor(tiles, dtype=torch.int32, device=device),
                               torch.tensor([used], dtype=torch.int32, device=device), counts=list(counts), even=even)
+
+
+def checked_linears(monkeypatch, fmt):
+    """Every linear layer that a model calls from now on is held to the oracle on its own input. (Whole forward passes
+    are not comparable: attention outputs that differ by one bf16 step in one place of ten move the logits of a small
+    random model by 10 to 30 per cent, because a code that changes changes by a quarter of its value.) Returns the list
+    of shapes that were checked."""
+    from arcticinference_b200 import ops
+    from arcticinference_b200.models.quant import Fp4Rows, Fp4Weight
+    inner, seen = ops.linear, []
+
+    def linear(x, w, *args, **kw):
+        y = inner(x, w, *args, **kw)
+        if isinstance(w, Fp4Weight):
+            assert not args and set(kw) <= {"bias", "sync"} and kw.get("sync") is None
+            xd = oracle_values(x.q, x.scale, x.row_scale, fmt) if isinstance(x, Fp4Rows) else oracle_rows(x, fmt)
+            wd = oracle_values(w.q, w.scale, w.row_scale, fmt)
+            want = xd @ wd.t()
+            if kw.get("bias") is not None:
+                want = want + kw["bias"].cpu().double()
+            bad = (y.cpu().double() - want).abs() > product_bound(xd, wd, want) + 2.0 ** -23
+            assert not bad.any(), (tuple(y.shape), bad.nonzero()[0].tolist())
+            seen.append((type(x).__name__, tuple(y.shape)))
+        return y
+
+    monkeypatch.setattr(ops, "linear", linear)
+    return seen
