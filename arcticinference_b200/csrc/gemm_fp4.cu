@@ -236,7 +236,7 @@ template <bool MX, bool PAIR, int SFB, int EPI>
 __global__ void __launch_bounds__(kF4Threads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                 const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
-                const Fp4GemmArgs p) {
+                const __grid_constant__ CUtensorMap tmap_x32, const Fp4GemmArgs p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
@@ -323,7 +323,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
             break;
           }
           // (pairs: one barrier, the even CTA's, collects the copies of both)
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), kCtas * stage_bytes);
+          const bool few = !PAIR && now.nrows <= 32;     // (an expert's few rows: a quarter of the box)
+          if (rank == 0)
+            mbar_arrive_expect_tx(full_bar(stage), few ? stage_bytes - p.b_bytes + 32u * 128u : kCtas * stage_bytes);
           const uint32_t full = PAIR ? map_to_cta(full_bar(stage), 0) : full_bar(stage);
           const uint32_t dst = smem_base + (uint32_t)stage * stage_bytes;
           const uint32_t sfa = dst + kF4ABytes + p.b_bytes;
@@ -334,7 +336,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
             tma_load_3d_pair(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, now.slot);
           } else {
             tma_load_3d(dst, &tmap_w, full, kb * 128, slice * 128, now.group);
-            tma_load_2d(dst + kF4ABytes, &tmap_x, full, kb * 128, row);
+            tma_load_2d(dst + kF4ABytes, few ? &tmap_x32 : &tmap_x, full, kb * 128, row);
             tma_load_3d(sfa, &tmap_sw, full, 0, kb * kTiles, now.group * p.w_row_tiles + slice);
             tma_load_3d(sfa + p.sfa_bytes, &tmap_sx, full, 0, kb * kTiles, now.slot);
           }
@@ -914,7 +916,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   const bool plain = act == 0 && residual == nullptr;
   const int step_tiles = mx ? 2 : 4, kblocks = (K + kF4StepCols - 1) / kF4StepCols;
   const int w_row_tiles = (N + 127) / 128, k_tiles = fp4_k_tiles(K, mx);
-  CUtensorMap tw, tx, tsw, tsx;
+  CUtensorMap tw, tx, tsw, tsx, tx32;
   // tokens of a tile (their rows of codes per CTA), row tiles that their scales lie in
   auto make_maps = [&](int x_rows, int sfb_tiles) {
     const uint64_t dims[3] = {(uint64_t)K / 2, (uint64_t)N, (uint64_t)groups};
@@ -1046,12 +1048,15 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   const long long total = (long long)(tiles != nullptr ? max_tiles : a.m_tiles) * a.n_tiles;
   if (total > 0x7fffffff) return -6;
 
-  if (!make_maps(pair ? a.bn / 2 : a.bn, a.sfb_tiles)) return -4;
+  if (!make_maps(pair ? a.bn / 2 : a.bn, a.sfb_tiles) ||
+      make_tmap_2d(&tx32, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K / 2, (uint64_t)ldx, 32, 128) != 0)
+    return -4;
   const size_t smem = (size_t)(a.stages * stage + header);
   const long long most = pair ? sms / 2 : sms;
   const dim3 grid((unsigned)((total < most ? total : most) * (pair ? 2 : 1)));
   auto go = [&](auto kernel) {
-    return launch_pdl_cluster(kernel, grid, dim3(kF4Threads), smem, stream, pair ? 2u : 1u, tw, tx, tsw, tsx, a);
+    return launch_pdl_cluster(kernel, grid, dim3(kF4Threads), smem, stream, pair ? 2u : 1u, tw, tx, tsw, tsx, tx32,
+                              a);
   };
   auto by_format = [&](auto nv, auto mxf) { return mx ? go(mxf) : go(nv); };
   cudaError_t e;

@@ -350,6 +350,7 @@ dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* 
   const int nvec = K / 8;
   const int padded = (group_rows + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
   const long long items = tiles != nullptr ? (long long)*num_tiles * kFp4TileRows : rows;
+  // (blockIdx.y: a part of the row)
   for (long long item = (long long)blockIdx.x * blockDim.y + threadIdx.y; item < items;
        item += (long long)gridDim.x * blockDim.y) {
     long long row = item, slot;
@@ -367,7 +368,7 @@ dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* 
                         fp4_scale_byte((int)(slot % kFp4TileRows));
     const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + row * ldq);
     uint4* o = reinterpret_cast<uint4*>(out + row * ldo);
-    for (int i0 = threadIdx.x; i0 < nvec; i0 += 4 * blockDim.x) {
+    for (int i0 = threadIdx.x + 4 * blockDim.x * blockIdx.y; i0 < nvec; i0 += 4 * blockDim.x * gridDim.y) {
       uint32_t byte[4], w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -516,7 +517,8 @@ int ab200_dequant_fp4(const void* q, long long ldq, const void* scale, const voi
   const int nvec = K / 8;
   const int across = nvec >= 1024 ? 256 : (((nvec + 3) / 4 + 31) / 32 * 32), down = 256 / across;
   const long long blocks = (rows + down - 1) / down;
-  const dim3 grid((unsigned)(tiles != nullptr ? 148 * 8 : blocks < 148ll * 256 ? blocks : 148ll * 256));
+  const dim3 grid((unsigned)(tiles != nullptr ? 148 * 8 : blocks < 148ll * 256 ? blocks : 148ll * 256),
+                  (unsigned)((nvec + 4 * across - 1) / (4 * across)));
   auto go = [&](auto kernel) {
     return launch_pdl(kernel, grid, dim3(across, down), 0, stream, reinterpret_cast<const uint8_t*>(q), ldq,
                       reinterpret_cast<const uint8_t*>(scale), reinterpret_cast<const float*>(row_scale),

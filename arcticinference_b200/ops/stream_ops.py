@@ -11,6 +11,7 @@ for a 32-bit model), its norm in those that normalise before the sublayer.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -33,17 +34,25 @@ class Gate:
 
     @staticmethod
     def of(gate) -> "Gate":
-        return gate if isinstance(gate, Gate) else Gate(gate)
+        return gate if isinstance(gate, Gate) else _named_gate(gate)
 
     @property
     def code(self) -> int:
-        return {"silu": 1, "gelu_tanh": 2, "clamped_swish": 3}[self.name]
+        return _GATE_CODES[self.name]
 
     def join(self, g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
         if self.name == "clamped_swish":
             g = g.clamp(max=self.limit)
             return g * torch.sigmoid(self.alpha * g) * (u.clamp(-self.limit, self.limit) + 1.0)
         return (F.silu(g) if self.name == "silu" else F.gelu(g, approximate="tanh")) * u
+
+
+_GATE_CODES = {"silu": 1, "gelu_tanh": 2, "clamped_swish": 3}
+
+
+@functools.lru_cache(maxsize=None)
+def _named_gate(name: str) -> Gate:
+    return Gate(name)
 
 
 def _nat():
