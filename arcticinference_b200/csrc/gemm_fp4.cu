@@ -232,8 +232,12 @@ __device__ __forceinline__ void f4_store32(const Fp4GemmArgs& p, const uint32_t 
   }
 }
 
+// Without pairs (experts with few rows) two CTAs share an SM: a tile has few steps, each of which costs some 0.3 us of
+// waits and issue whatever it moves, and one CTA's accumulator is drained beside the other's products. 64 experts of
+// 2 x 1408, mxfp4, gate / up and down in us, one CTA an SM and two: 768 rows 36.9 + 22.0 and 36.2 + 23.6, 6144 rows 50.6
+// + 32.8 and 47.7 + 30.6, 20000 rows 105 + 63 and 88 + 56.
 template <bool MX, bool PAIR, int SFB, int EPI>
-__global__ void __launch_bounds__(kF4Threads, 1)
+__global__ void __launch_bounds__(kF4Threads, PAIR ? 1 : 2)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                 const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx,
                 const __grid_constant__ CUtensorMap tmap_x32, const Fp4GemmArgs p) {
@@ -247,6 +251,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   }
   constexpr int kTiles = MX ? 2 : 4;      // scale tiles of a step
   constexpr int kCtas = PAIR ? 2 : 1;
+  constexpr int kAccs = PAIR ? 2 : 1;
+  constexpr uint32_t kColumns = PAIR ? 512 : 256, kScaleAt = PAIR ? kF4ScaleAt : 128u;
   const uint32_t stage_bytes = kF4ABytes + p.b_bytes + p.sfa_bytes + p.sfb_bytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * stage_bytes);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kF4MaxStages + 5);
@@ -282,10 +288,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   }
   if (warp == 1) {
     if (PAIR) {
-      tmem_alloc_pair(smem_u32(tmem_slot), 512);
+      tmem_alloc_pair(smem_u32(tmem_slot), kColumns);
       tmem_relinquish_pair();
     } else {
-      tmem_alloc(smem_u32(tmem_slot), 512);
+      tmem_alloc(smem_u32(tmem_slot), kColumns);
       tmem_relinquish();
     }
   }
@@ -387,7 +393,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         const uint32_t idesc = make_idesc_fp4(128 * kCtas, n, MX, 0), idesc_hi = make_idesc_fp4(128 * kCtas, n, MX, 2);
         const uint32_t d_tmem = __shfl_sync(0xffffffffu, tm + f4_accumulator(acc, t.nrows), 0);
         for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (steps >= kSets) {
+          // (a ring of no more stages than sets: the stage's own wait says so)
+          if (steps >= kSets && p.stages > kSets) {
             const bool wrapped = stage < kSets;
             if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage - kSets + (wrapped ? p.stages : 0)),
                                                    phase ^ (wrapped ? 1u : 0u), abort_flag, p.status, 1620 + stage, kb))) {
@@ -404,7 +411,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           const uint64_t b_desc = a_desc + (uint64_t)(kF4ABytes / 16);
           const uint64_t sa_desc = s0 + (uint64_t)stage * stage_step;
           const uint64_t sb_desc = sa_desc + (uint64_t)(kSfaBytes / 16);
-          const uint32_t sfa = tm + kF4ScaleAt + set * kSetColumns, sfb = sfa + 16u;
+          const uint32_t sfa = tm + kScaleAt + set * kSetColumns, sfb = sfa + 16u;
           const uint32_t sfb_first = sfb + shift;
           if (elect_one()) {
 #pragma unroll
@@ -439,8 +446,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           }
         }
         if (!ok) break;
-        acc ^= 1;
-        if (acc == 0) side_phase ^= 1u;
+        if (++acc == kAccs) {
+          acc = 0;
+          side_phase ^= 1u;
+        }
       }
     }
   } else {
@@ -491,35 +500,57 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         break;
       tc_fence_after();
       const uint32_t t_addr = tmem_base + f4_accumulator(acc, t.nrows) + ((uint32_t)(quad * 32) << 16);
-      // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and both
-      // handed back as soon as they are in registers.
-      const bool wide = t.nrows > (int)kF4Middle;
-      const int first = wide && acc == 0 ? 128 : 0;
-      for (int part = 0; part < (wide ? 2 : 1); ++part) {
-        const int c0 = (part == 0 ? first : 128 - first) + 32 * half;
-        const bool any0 = c0 < t.nrows && feature0 < p.N, any1 = c0 + 64 < t.nrows && feature0 < p.N;
-        uint32_t r[4][16];
-        __syncwarp();
-        if (any0) {
-          tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
-          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
-        }
-        if (any1) {
-          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + 64u, r[2]);
-          tmem_ld_frag_x4(t_addr + (uint32_t)c0 + 64u + (16u << 16), r[3]);
-        }
+      if (!PAIR) {
+        // (half the registers: 32 tokens at a time)
+        coming_factors = fetch(coming);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < 2 ? any0 : any1) tmem_ld_wait_dep(r[i]);
-        hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
-        if (part == 0) coming_factors = fetch(coming);
-        const bool upper = c0 >= 128;
-        if (any0) f4_store32<EPI>(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[2] : fc.gx[0], lane);
-        if (any1)
-          f4_store32<EPI>(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[3] : fc.gx[1], lane);
+        for (int q = 0; q < 2; ++q) {
+          const int c0 = 32 * half + 64 * q;
+          const bool any = c0 < t.nrows && feature0 < p.N;
+          uint32_t r[2][16];
+          __syncwarp();
+          if (any) {
+            tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
+            tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
+            tmem_ld_wait_dep(r[0]);
+            tmem_ld_wait_dep(r[1]);
+          }
+          if (q == 1) hand_back(side_bar(acc));
+          if (any) f4_store32<EPI>(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, fc.gx[q], lane);
+        }
+      } else {
+              // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and both
+        // handed back as soon as they are in registers.
+        const bool wide = t.nrows > (int)kF4Middle;
+        const int first = wide && acc == 0 ? 128 : 0;
+        for (int part = 0; part < (wide ? 2 : 1); ++part) {
+          const int c0 = (part == 0 ? first : 128 - first) + 32 * half;
+          const bool any0 = c0 < t.nrows && feature0 < p.N, any1 = c0 + 64 < t.nrows && feature0 < p.N;
+          uint32_t r[4][16];
+          __syncwarp();
+          if (any0) {
+            tmem_ld_frag_x4(t_addr + (uint32_t)c0, r[0]);
+            tmem_ld_frag_x4(t_addr + (uint32_t)c0 + (16u << 16), r[1]);
+          }
+          if (any1) {
+            tmem_ld_frag_x4(t_addr + (uint32_t)c0 + 64u, r[2]);
+            tmem_ld_frag_x4(t_addr + (uint32_t)c0 + 64u + (16u << 16), r[3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < 2 ? any0 : any1) tmem_ld_wait_dep(r[i]);
+          hand_back(wide && part == 0 ? middle_bar : side_bar(acc));
+          if (part == 0) coming_factors = fetch(coming);
+          const bool upper = c0 >= 128;
+          if (any0) f4_store32<EPI>(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[2] : fc.gx[0], lane);
+          if (any1)
+            f4_store32<EPI>(p, r[2], r[3], my_stage, c0 + 64, t.row0, t.nrows, feature0, fc.ft, upper ? fc.gx[3] : fc.gx[1], lane);
+        }
       }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
+      if (++acc == kAccs) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
     }
   }
 
@@ -528,8 +559,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   if (PAIR) cluster_sync();   // neither CTA leaves while the other may still signal it
   if (warp == 1) {
     tc_fence_after();
-    if (PAIR) tmem_dealloc_pair(tmem_base, 512);
-    else tmem_dealloc(tmem_base, 512);
+    if (PAIR) tmem_dealloc_pair(tmem_base, kColumns);
+    else tmem_dealloc(tmem_base, kColumns);
   }
 }
 
@@ -1043,7 +1074,8 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   a.status = status;
   const uint64_t stage = kF4ABytes + a.b_bytes + a.sfa_bytes + a.sfb_bytes;
   const uint64_t header = 256 + kF4EpilogueWarps * kF4StoreBytes;
-  a.stages = (int)((227 * 1024 - header) / stage);
+  const int per_sm = pair ? 1 : 2;
+  a.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - header) / stage);
   if (a.stages > kF4MaxStages) a.stages = kF4MaxStages;
   const long long total = (long long)(tiles != nullptr ? max_tiles : a.m_tiles) * a.n_tiles;
   if (total > 0x7fffffff) return -6;
@@ -1052,7 +1084,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
       make_tmap_2d(&tx32, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K / 2, (uint64_t)ldx, 32, 128) != 0)
     return -4;
   const size_t smem = (size_t)(a.stages * stage + header);
-  const long long most = pair ? sms / 2 : sms;
+  const long long most = pair ? sms / 2 : 2 * sms;
   const dim3 grid((unsigned)((total < most ? total : most) * (pair ? 2 : 1)));
   auto go = [&](auto kernel) {
     return launch_pdl_cluster(kernel, grid, dim3(kF4Threads), smem, stream, pair ? 2u : 1u, tw, tx, tsw, tsx, tx32,
