@@ -40,6 +40,7 @@ struct Fp4GemmArgs {
   uint32_t b_bytes, sfa_bytes, sfb_bytes;
   int sfb_tiles;           // row tiles that the scales of a tile's tokens lie in
   int w_row_tiles;         // row tiles of scales per matrix
+  int groups;
   int list_tiles;          // tiles of the list that are taken together: two where groups have an even number
   int act;
   GateParams gate;
@@ -72,6 +73,13 @@ __device__ __forceinline__ F4Work f4_work(const Fp4GemmArgs& p, int w) {
     r.row0 = t.y;
     r.nrows = t.z;
     if (p.list_tiles == 2) r.nrows += p.tiles[mt + 1].z;
+    // (a list made for other rows or experts reaches beyond neither)
+    r.nrows = min(min(r.nrows, p.bn), p.M - r.row0);
+    if ((unsigned)r.group >= (unsigned)p.groups || r.row0 < 0) {
+      r.group = 0;
+      r.row0 = 0;
+      r.nrows = 0;
+    }
     r.slot = mt;
     r.shift = 0;
     return r;
@@ -302,7 +310,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();   // (tensor memory is owned)
   pdl_wait();
-  const int total_work = (p.tiles != nullptr ? *p.num_tiles / p.list_tiles : p.m_tiles) * p.n_tiles;
+  const int total_work =
+      (p.tiles != nullptr ? min(*p.num_tiles, p.m_tiles) / p.list_tiles : p.m_tiles) * p.n_tiles;
   const int first_work = (int)blockIdx.x / kCtas, work_step = (int)gridDim.x / kCtas;
   auto work = [&](int w) {
     F4Work none = {};
@@ -791,10 +800,9 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
       bias[e] = 0.f;
     }
     if (mine_too) {
-      if (p.w_scale != nullptr) {
-        const float4 a = load4(p.w_scale + f), b = load4(p.w_scale + f + 4);
-        h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
-        h[4] = b.x; h[5] = b.y; h[6] = b.z; h[7] = b.w;
+      if (p.w_scale != nullptr) {   // (on any 4-byte boundary)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = p.w_scale[f + e];
       }
       if (p.bias != nullptr) {
 #pragma unroll
@@ -1053,12 +1061,13 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
       }
     }
   }
-  a.m_tiles = (int)((M + a.bn - 1) / a.bn);
+  a.m_tiles = tiles != nullptr ? max_tiles : (int)((M + a.bn - 1) / a.bn);
   a.sfb_tiles = a.bn > 128 ? 2 : 1;
   a.b_bytes = (uint32_t)(pair ? a.bn / 2 : a.bn) * 128;
   a.sfa_bytes = (uint32_t)step_tiles * kFp4ScaleTile;
   a.sfb_bytes = a.sfa_bytes * (uint32_t)a.sfb_tiles;
   a.w_row_tiles = w_row_tiles;
+  a.groups = groups;
   a.act = gate != 0 ? gate : act;
   a.gate.limit = gate_limit;
   a.gate.alpha = gate_alpha;
@@ -1077,7 +1086,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   const int per_sm = pair ? 1 : 2;
   a.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - header) / stage);
   if (a.stages > kF4MaxStages) a.stages = kF4MaxStages;
-  const long long total = (long long)(tiles != nullptr ? max_tiles : a.m_tiles) * a.n_tiles;
+  const long long total = (long long)a.m_tiles * a.n_tiles;
   if (total > 0x7fffffff) return -6;
 
   if (!make_maps(pair ? a.bn / 2 : a.bn, a.sfb_tiles) ||

@@ -21,9 +21,9 @@
 // its side. Divisions rounded to the last bit gave the same results in twice the time. (Which of
 // its two codes a zero gets says nothing.)
 //
-// One CTA (or warp) per row, the row in registers between the maximum and the rounding: one pass over memory. Eight columns
-// per thread and step: 16-byte loads, 4-byte stores of codes; the lanes of a block share its maximum by shuffles and
-// four blocks' scales leave as one word. The values are the bf16 numbers that the unfused kernel would have
+// One CTA (or warp) per row, the row in registers between the maximum and the rounding: one pass over memory. 16-byte
+// loads, 4 or 8-byte stores of codes; the lanes of a block share its maximum by shuffles and four blocks' scales leave as
+// one word. The values are the bf16 numbers that the unfused kernel would have
 // stored (same order of the norm's sum), so fused and unfused paths agree bit for bit.
 
 #include <cuda_fp8.h>
@@ -172,7 +172,7 @@ __device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int lane)
     int in = -1;
     if (i + lane < step && at < n) {
       const int4 t = p.tiles[at];
-      if (row >= t.y && row < t.y + t.z) in = row - t.y;
+      if (row >= t.y && row < t.y + min(t.z, kFp4TileRows)) in = row - t.y;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, in >= 0);
     if (hit != 0u) {
@@ -183,20 +183,25 @@ __device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int lane)
   return -1;
 }
 
-// WARP: a warp per row and no barrier, for rows that 32 threads hold; otherwise a block per row.
+// WARP: a warp per row and no barrier, for rows that 32 threads hold; otherwise a block per row. A thread takes pieces
+// of 16 columns, whose one scale (nvfp4) it then computes alone: 8192 x 4096 took 16.1 us with pieces of 8, and the
+// instructions bound it. (The norm keeps pieces of 8, in which the unfused kernel adds.)
 template <int SRC, bool MX, int VPT, bool WARP>
 __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
   pdl_wait();
   pdl_trigger();
   __shared__ uint32_t red[32];
   __shared__ int block_slot;
-  constexpr int kBlockVecs = MX ? 4 : 2;          // lanes of a block
-  constexpr int kTileVecs = 4 * kBlockVecs;       // lanes of a word of scales
+  constexpr int kPer = SRC == kFp4Norm || VPT == 1 ? 1 : 2;        // eight columns each in a piece
+  constexpr int kPieces = VPT / kPer;
+  constexpr int kBlockLanes = (MX ? 4 : 2) / kPer;                 // lanes of a block
+  constexpr int kTileLanes = 4 * kBlockLanes;                      // lanes of a word of scales
   const int lane = threadIdx.x & 31;
   const int tid = WARP ? lane : (int)threadIdx.x, threads = WARP ? 32 : (int)blockDim.x;
   const int row = WARP ? (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) : (int)blockIdx.x;
   if (WARP && row >= p.M) return;
-  const int nvec = p.K / 8, all = p.k_tiles * kTileVecs;
+  const int nvec = p.K / 8, pieces = nvec / kPer, all = p.k_tiles * kTileLanes;
+  auto vec_of = [&](int j) { return (tid + j / kPer * threads) * kPer + j % kPer; };
   // everything that is read is requested first
   uint4 raw[VPT], other[SRC == kFp4Plain ? 1 : VPT], wraw[SRC == kFp4Norm ? VPT : 1];
   const uint4* xr = reinterpret_cast<const uint4*>(p.x + (long long)row * p.ldx);
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
                                                        : nullptr;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int i = tid + j * threads;
+    const int i = vec_of(j);
     raw[j] = make_uint4(0, 0, 0, 0);
     if (SRC != kFp4Plain) other[j] = make_uint4(0, 0, 0, 0);
     if (SRC == kFp4Norm) wraw[j] = make_uint4(0, 0, 0, 0);
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
     float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int i = tid + j * threads;
+      const int i = vec_of(j);
       float v[8];
       fq_unpack8(raw[j], v);
       if (rr != nullptr) {
@@ -275,12 +280,13 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
       raw[j] = fq_pack8(v);
     }
   }
-  uint32_t top[VPT], most = 0;
+  uint32_t top[kPieces], most = 0;
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    uint32_t t = fq_top8(raw[j]);
-    t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
-    if (MX) t = max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+  for (int j = 0; j < kPieces; ++j) {
+    uint32_t t = fq_top8(raw[kPer * j]);
+    if (kPer == 2) t = max(t, fq_top8(raw[kPer * j + kPer - 1]));
+    if (kBlockLanes >= 2) t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+    if (kBlockLanes >= 4) t = max(t, __shfl_xor_sync(0xffffffffu, t, 2));
     top[j] = t;
     most = max(most, t);
   }
@@ -304,8 +310,9 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] *= 0x1p+60f;
         raw[j] = fq_pack8(v);
-        top[j] = __float_as_uint(__uint_as_float(top[j] << 16) * 0x1p+60f) >> 16;
       }
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) top[j] = __float_as_uint(__uint_as_float(top[j] << 16) * 0x1p+60f) >> 16;
     }
   }
   if (slot < 0) return;
@@ -313,31 +320,44 @@ __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
   uint8_t* sr = p.scale + (long long)(slot / kFp4TileRows) * p.k_tiles * kFp4ScaleTile +
                 fp4_scale_byte(slot % kFp4TileRows);
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
+  for (int j = 0; j < kPieces; ++j) {
     const int i = tid + j * threads;
-    uint32_t byte, code;
+    uint32_t byte, code[kPer];
+    float r;
+    bool some;
     if (MX) {
       const int e = max((int)(top[j] >> 7) - 2, 0);      // the exponent's field
-      byte = top[j] < 0x7f80u ? (uint32_t)e : 0xffu;
-      code = top[j] < 0x7f80u ? fq_codes8<true>(raw[j], fp4_pow2(127 - e)) : 0u;
+      some = top[j] < 0x7f80u;
+      byte = some ? (uint32_t)e : 0xffu;
+      r = fp4_pow2(127 - e);
     } else {
       const __half t = __float2half_rn(__uint_as_float(top[j] << 16) * up * (1.f / 6.f));
       byte = most < 0x7f80u ? (uint32_t)__nv_cvt_halfraw_to_fp8(t, __NV_SATFINITE, __NV_E4M3) : 0u;
-      code = byte != 0u ? fq_codes8<false>(raw[j], up * rcp_approx(e4m3_value(byte))) : 0u;
+      some = byte != 0u;
+      r = up * rcp_approx(e4m3_value(byte));
     }
-    if (i < nvec) qr[i] = code;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const uint32_t c = fq_codes8<MX>(raw[kPer * j + e], r);
+      code[e] = some ? c : 0u;
+    }
+    if (i < pieces) {
+      if (kPer == 2) *reinterpret_cast<uint2*>(qr + 2 * i) = make_uint2(code[0], code[kPer - 1]);
+      else qr[i] = code[0];
+    }
     // the scales of four blocks in one word; blocks behind the row's end have the scale zero
-    if (i >= nvec) byte = 0u;
-    const uint32_t b1 = __shfl_down_sync(0xffffffffu, byte, kBlockVecs);
+    if (i >= pieces) byte = 0u;
+    const uint32_t b1 = __shfl_down_sync(0xffffffffu, byte, kBlockLanes);
     const uint32_t two = byte | (b1 << 8);
-    const uint32_t four = two | (__shfl_down_sync(0xffffffffu, two, 2 * kBlockVecs) << 16);
-    if (i < all && (i % kTileVecs) == 0)
-      *reinterpret_cast<uint32_t*>(sr + (long long)(i / kTileVecs) * kFp4ScaleTile) = four;
+    const uint32_t four = two | (__shfl_down_sync(0xffffffffu, two, 2 * kBlockLanes) << 16);
+    if (i < all && (i % kTileLanes) == 0)
+      *reinterpret_cast<uint32_t*>(sr + (long long)(i / kTileLanes) * kFp4ScaleTile) = four;
   }
 }
 
 // Eight numbers per thread and step, four steps on their way together; threadIdx.y: rows of a block. Rows of a weight of
-// several groups: each group's scale tiles begin anew.
+// several groups: each group's scale tiles begin anew. (16 numbers a thread would halve the work on scales, but a store
+// instruction then leaves half of every sector to the next one: 20.6 instead of 15.0 us for 8192 x 4096.)
 template <bool MX>
 __global__ void __launch_bounds__(256)
 dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ scale,
@@ -357,8 +377,8 @@ dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* 
     if (tiles != nullptr) {
       const int4 t = tiles[item / kFp4TileRows];
       const int in = (int)(item % kFp4TileRows);
-      if (in >= t.z) continue;
       row = t.y + in;
+      if (in >= t.z || row < 0 || row >= rows) continue;
       slot = item;
     } else {
       slot = row / group_rows * padded + row % group_rows;
@@ -382,10 +402,15 @@ dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* 
         float s;
         if (MX) s = byte[j] == 0xffu ? __uint_as_float(0x7fffffffu) : fp4_pow2((int)byte[j] - 127);
         else s = e4m3_value(byte[j]);
+        const float2 f = make_float2(s * g, s * g);
         float v[8];
         fq_values8(w[j], v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = v[k] * s * g;
+        for (int k = 0; k < 4; ++k) {
+          const float2 t = mul_x2(make_float2(v[2 * k], v[2 * k + 1]), f);
+          v[2 * k] = t.x;
+          v[2 * k + 1] = t.y;
+        }
         if (i < nvec) o[i] = fq_pack8(v);
       }
     }

@@ -408,3 +408,98 @@ def test_refusals():
             raise AssertionError("case %d was not refused" % i)
     torch.cuda.synchronize()
     ops.check_status()
+
+
+# ------------------------------------------------------------------------ calls at the edges of what is allowed
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_lists_that_reach_beyond_the_rows(fmt):
+    """A routing of more rows than there are: what is there is served, nothing beyond it is touched."""
+    counts = [100, 60, 0, 90]
+    w4 = quant.quantize_weight_fp4(_rand(4, 64, 96, seed=1, scale=0.1).cuda(), fmt)
+    x = _rand(250, 96, seed=2)
+    whole = stream_ops.grouped_linear(x.cuda(), w4, routing_of(counts, "cuda"))
+    for even in (False, True):
+        r = routing_of(counts, "cuda", even)
+        for n in (250, 180, 110, 3):
+            buf = torch.empty(n + 8, 96, dtype=torch.bfloat16, device="cuda")
+            buf[:n] = x[:n].cuda()
+            assert torch.equal(stream_ops.grouped_linear(buf[:n], w4, r), whole[:n])
+            q = ops.quant_fp4(buf[:n], fmt, r)
+            assert torch.equal(q.dequantize(), ops.quant_fp4(buf[:n], fmt).dequantize())
+    r = routing_of(counts, "cuda")
+    r.tiles[2:, 0] = 9                                  # no such expert: left out
+    stream_ops.grouped_linear(x.cuda(), w4, r)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M", [3, 100, 300])
+def test_factors_and_bias_on_any_boundary(M):
+    N, K = 264, 2048
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=0.03).cuda(), "nvfp4")
+    g = torch.cat([torch.zeros(1), 0.5 + torch.rand(N, generator=torch.Generator().manual_seed(3))]).cuda()[1:]
+    bias = torch.cat([torch.zeros(1, dtype=torch.bfloat16), _rand(N, seed=4)]).cuda()[1:]
+    assert g.data_ptr() % 8 and bias.data_ptr() % 4
+    x = _rand(M, K, seed=2)
+    got = ops.linear(x.cuda(), quant.Fp4Weight(w4.q, w4.scale, g, "nvfp4"), bias=bias)
+    assert torch.equal(got, ops.linear(x.cuda(), quant.Fp4Weight(w4.q, w4.scale, g.clone(), "nvfp4"), bias=bias.clone()))
+    _check(x, quant.Fp4Weight(w4.q, w4.scale, g, "nvfp4"), "nvfp4", bias=bias.cpu())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_wider_than_the_quantisers_take(fmt):
+    """Rows that were quantised elsewhere may be longer than 32768."""
+    K, N, M = 33024, 16, 130
+    x, w = (torch.randint(0, 256, (r, K // 2), generator=torch.Generator().manual_seed(r), dtype=torch.uint8) for r in (M, N))
+    tile = lambda r: torch.full(quant.fp4_scale_tiles(r, K, fmt), 48 if fmt == "nvfp4" else 120, dtype=torch.uint8)
+    xr, wr = quant.Fp4Rows(x, tile(M), None, fmt), quant.Fp4Weight(w, tile(N), None, fmt)
+    xd, wd = (oracle_values(t.q, t.scale, None, fmt) for t in (xr, wr))
+    got = ops.linear(quant.Fp4Rows(x.cuda(), tile(M).cuda(), None, fmt), quant.Fp4Weight(w.cuda(), tile(N).cuda(), None, fmt))
+    y = xd @ wd.t()
+    assert ((got.cpu().double() - y).abs() <= product_bound(xd, wd, y)).all()
+    with pytest.raises(ValueError):
+        ops.linear(torch.zeros(2, K, dtype=torch.bfloat16, device="cuda"), quant.Fp4Weight(w.cuda(), tile(N).cuda(), None, fmt))
+
+
+def test_captured_calls_share_nothing():
+    """Two graphs of the same layer replayed in turn, beside eager calls, on inputs that change."""
+    w4 = quant.quantize_weight_fp4(_rand(520, 4096, seed=1, scale=0.02).cuda(), "nvfp4")
+    xs = [_rand(m, 4096, seed=m).cuda() for m in (7, 140)]
+    for x in xs:
+        ops.linear(x, w4)
+    torch.cuda.synchronize()
+    graphs = []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.linear(x, w4)
+        graphs.append((g, x, y))
+    for step in range(4):
+        for g, x, y in graphs:
+            x.copy_(_rand(*x.shape, seed=10 * step + x.shape[0]))
+            g.replay()
+        for g, x, y in graphs:
+            assert torch.equal(ops.linear(x, w4), y)
+    ops.check_status()
+
+
+def test_input_that_the_output_overwrites():
+    w4 = quant.quantize_weight_fp4(_rand(256, 256, seed=1, scale=0.1).cuda(), "mxfp4")
+    for M in (5, 300):
+        x = _rand(M, 256, seed=2).cuda()
+        want = ops.linear(x, w4)
+        assert ops.linear(x, w4, out=x) is x and torch.equal(x, want)
+
+
+def test_long_offsets():
+    """Rows and weights whose elements lie more than 2^31 bytes apart."""
+    K, N, M = 64, 136, 70
+    big = torch.empty(M * (1 << 25), dtype=torch.bfloat16, device="cuda").view(M, 1 << 25)      # 4.7 GB
+    x = big[:, :K]
+    x.copy_(_rand(M, K, seed=2))
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=0.1).cuda(), "nvfp4")
+    out = big[:, 1024:1024 + N]
+    assert torch.equal(ops.linear(x, w4, out=out), ops.linear(x.contiguous(), w4))
+    res = big[:, 4096:4096 + N]
+    res.copy_(_rand(M, N, seed=3))
+    assert torch.equal(ops.linear(x, w4, residual=res), ops.linear(x.contiguous(), w4, residual=res.contiguous()))
+    ops.check_status()
