@@ -505,6 +505,10 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
     on_device_of(wq, xq);
     M = o.rows;
   }
+  TORCH_CHECK_VALUE(K > 0, "4-bit product: rows without columns");
+  TORCH_CHECK_VALUE(status.scalar_type() == at::kInt && status.is_contiguous() && status.numel() >= 8,
+                    "4-bit product: status is int32 [8]");
+  on_device_of(wq, status);
   const bool grouped = row_tiles > 0;
   TORCH_CHECK_VALUE(grouped == (wq.dim() == 3), "4-bit product: several matrices go with a routing");
   TORCH_CHECK_VALUE(N % (gate ? 32 : 8) == 0, "4-bit product: N a multiple of ", gate ? 32 : 8, ", got ", N);
@@ -522,7 +526,10 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
                       "4-bit product: bias is bf16 [", N, "]");
     on_device_of(wq, bias);
   }
-  if (out.defined()) matrix(out, "out");
+  if (out.defined()) {
+    matrix(out, "out");
+    TORCH_CHECK_VALUE(M <= 1 || out.stride(0) >= width, "4-bit product: rows of out overlap");
+  }
   else out = at::empty({M, width}, wq.options().dtype(at::kBFloat16));
   if (M == 0 || N == 0) return;
   if (has(x0)) {

@@ -156,6 +156,7 @@ def linear_fp4(x, w, bias=None, residual=None, act=None, out=None) -> torch.Tens
 def _linear_ref(x, w, bias, residual, act, out):
     from ..models import quant
     N, K = w.shape
+    _need(K > 0, "linear_fp4: rows without columns")
     _need(len(x.shape) == 2 and x.shape[1] == K, "linear_fp4: rows %s and weight %s", tuple(x.shape), (N, K))
     M = x.shape[0]
     for name, t, shape in (("bias", bias, (N,)), ("residual", residual, (M, N)), ("out", out, (M, N))):

@@ -151,3 +151,11 @@ def test_no_rows():
     w4 = quant.quantize_weight_fp4(_rand(32, 64), "mxfp4")
     x = torch.empty(0, 64, dtype=torch.bfloat16)
     assert ops.linear(x, w4).shape == (0, 32) and ops.quant_fp4(x, "nvfp4").dequantize().shape == (0, 64)
+
+
+def test_products_without_columns_are_refused():
+    scale = torch.empty(1, 0, 512, dtype=torch.uint8)
+    x = quant.Fp4Rows(torch.empty(4, 0, dtype=torch.uint8), scale, None, "mxfp4")
+    w = quant.Fp4Weight(torch.empty(40, 0, dtype=torch.uint8), scale, None, "mxfp4")
+    with pytest.raises(ValueError):
+        ops.linear(x, w)

@@ -503,3 +503,31 @@ def test_long_offsets():
     res.copy_(_rand(M, N, seed=3))
     assert torch.equal(ops.linear(x, w4, residual=res), ops.linear(x.contiguous(), w4, residual=res.contiguous()))
     ops.check_status()
+
+
+def test_refused_outputs_and_widths():
+    x, w4 = _rand(4, 64).cuda(), quant.quantize_weight_fp4(_rand(40, 64).cuda(), "nvfp4")
+    byte = dict(dtype=torch.uint8, device="cuda")
+    none_x = quant.Fp4Rows(torch.empty(4, 0, **byte), torch.empty(1, 0, 512, **byte), None, "mxfp4")
+    none_w = quant.Fp4Weight(torch.empty(40, 0, **byte), torch.empty(1, 0, 512, **byte), None, "mxfp4")
+    one = torch.zeros(1, 40, dtype=torch.bfloat16, device="cuda")
+    table = torch.ops.arcticinference_b200
+    bad = [
+        lambda: ops.linear(none_x, none_w),                       # no columns
+        lambda: ops.linear(x, w4, out=one.expand(4, 40)),          # four rows in one place
+        lambda: ops.linear(x, w4, out=torch.zeros(200, dtype=torch.bfloat16, device="cuda").as_strided((4, 40), (32, 1))),
+        lambda: table.fp4_linear(x, None, None, None, w4.q, w4.scale, w4.row_scale, 0, None, None, 0,
+                                 torch.zeros(1, dtype=torch.int32, device="cuda")),
+        lambda: table.fp4_linear(x, None, None, None, w4.q, w4.scale, w4.row_scale, 0, None, None, 0,
+                                 torch.zeros(8, dtype=torch.int32)),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            raise AssertionError("case %d was not refused" % i)
+    # (one row may have any stride; a residual may be one row for all)
+    ops.linear(x[:1], w4, out=one)
+    r = _rand(1, 40, seed=3).cuda()
+    assert torch.equal(ops.linear(x, w4, residual=r.expand(4, 40)), ops.linear(x, w4, residual=r.repeat(4, 1)))
+    torch.cuda.synchronize()
+    ops.check_status()
