@@ -10,6 +10,10 @@
 // 256 columns of both operands (128 bytes a row, 128-byte swizzle) and their scale tiles. One warp copies a stage's
 // scales to tensor memory (sets used in turn) and issues the products into one of two accumulators;
 // eight warps drain the other one.
+//
+// One B200, nvfp4: 8192 x 28672 x 4096 370 to 380 us (5.1 to 5.2 PFLOP/s; mxfp4 343 to 352, 5.5 to 5.6), bound by shared memory
+// (608 cycles of copies and operands per 512 of products); 49152 rows of 64 experts, 2 x 1408 from 2048, 149 to 154 us, bound
+// by the boundaries of tiles of eight steps; 768 rows 39 us, the weights at 5.3 TB/s.
 
 #include <string.h>
 
@@ -528,8 +532,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           if (any) f4_store32<EPI>(p, r[0], r[1], my_stage, c0, t.row0, t.nrows, feature0, fc.ft, fc.gx[q], lane);
         }
       } else {
-              // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and both
-        // handed back as soon as they are in registers.
+        // 128 tokens at a time, alternate groups of 32 for the quadrant's two warps. The middle columns first, and
+        // both handed back as soon as they are in registers.
         const bool wide = t.nrows > (int)kF4Middle;
         const int first = wide && acc == 0 ? 128 : 0;
         for (int part = 0; part < (wide ? 2 : 1); ++part) {
@@ -578,8 +582,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 // tiles are fewer than the SMs, a part of K: the CTAs of a cluster that share a tile send each other their fp32 sums,
 // slices of 16 features, and each adds those of its own slices in the order of K and stores them. The sums go into
 // the sender's shared memory first and from there as bulk copies that complete on a barrier of the receiver; stores
-// into another CTA's memory, eight bytes a lane, and a cluster barrier on either side took 5.5 us for 128 tokens. The weights' first steps are requested into L2 before the wait for the kernel ahead, whose tail (the rows'
-// quantisation) they cover: a prefetch changes no value, whoever has written them.
+// into another CTA's memory, eight bytes a lane, and a cluster barrier on either side took 5.5 us for 128 tokens. The
+// weights' first steps are requested into L2 before the wait for the kernel ahead, whose tail (the rows' quantisation)
+// they cover: a prefetch changes no value, whoever has written them. One token, nvfp4: 28672 x 4096 12.9 us (5.1 TB/s),
+// 4096 x 14336 10.4 us (3.2; 25.4 before K was split), 4096 x 4096 5.2 us; 128 tokens 15.2, 12.7 and 7.9 us.
 struct Fp4FewArgs {
   int N, M, kblocks, splits, per_split, stages;
   uint32_t b_bytes, columns, scale_at, recv_at;
@@ -1047,8 +1053,8 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   a.list_tiles = even != 0 ? 2 : 1;
   a.bn = 128 * a.list_tiles;
   if (tiles == nullptr) {
-    // Width of the token tiles: waves of pairs times what 16 steps of a tile take (measured with N = 28672, M = 1500: 77,
-    // 87, 111 and 206 us for 256, 192, 128 and 64; M = 300, N = 4096: 11.0, 10.5, 9.6, 13.9).
+    // Width of the token tiles: waves of pairs times what 16 steps of a tile take (measured with N = 28672, M = 1500: 75,
+    // 85, 110 and 203 us for 256, 192, 128 and 64; M = 300, N = 4096: 11.0, 10.4, 9.6, 13.8).
     const int width[4] = {256, 192, 128, 64};
     const double us[4] = {7.7, 6.7, 5.9, 5.6};
     double best = 1e30;
