@@ -370,6 +370,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
                      int N, int K, int groups, int fmt, const void* bias, const void* residual, long long ldr, int act,
                      int gate, float gate_limit, float gate_alpha, const void* tiles, const void* num_tiles,
                      int max_tiles, int even, int* status, cudaStream_t stream);
+int ab200_linear_fp4_plan(long long M, int N, int K, int fmt, int sms, int* splits, int* columns, long long* smem);
 
 #ifdef __cplusplus
 }

@@ -907,11 +907,73 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
   }
 }
 
+struct Fp4FewPlan {
+  int x_rows, splits, per_split, stages, columns, scale_at;
+  uint64_t recv_at, smem;
+};
+
+// Parts of K, stages and memory of a product of M tokens, at most kFewTokens.
+static Fp4FewPlan fp4_few_plan(int M, int N, int K, bool mx, int sms) {
+  Fp4FewPlan f;
+  const int step_tiles = mx ? 2 : 4, kblocks = (K + kF4StepCols - 1) / kF4StepCols, w_row_tiles = (N + 127) / 128;
+  f.x_rows = (M + 15) / 16 * 16;
+  const uint64_t stage = kF4ABytes + (uint64_t)f.x_rows * 128 + 2ull * step_tiles * kFp4ScaleTile;
+  // More tiles than SMs: two CTAs on each, with half of its shared and tensor memory. Fewer: a tile's steps are
+  // split.
+  const int per_sm = w_row_tiles > sms ? 2 : 1;
+  // (0.31 us a step; the exchange 1.0 to 2.0 us between two CTAs, 1.8 to 3.7 between four, by the tokens: 4096 x 4096,
+  // 1, 64 and 128 tokens 7.2, 7.5, 8.5 us unsplit, 5.7, 6.5, 7.8 with two parts, 5.2, 6.6, 8.4 with four; eight never paid)
+  f.splits = 1;
+  double least = 0.31 * kblocks;
+  for (int parts = 2; parts <= 4 && w_row_tiles * parts <= sms; parts *= 2) {
+    const double t = 0.31 * kblocks / parts + (parts == 2 ? 1.0 + 0.008 * M : 1.8 + 0.015 * M);
+    if (t < least) {
+      least = t;
+      f.splits = parts;
+    }
+  }
+  f.per_split = (kblocks + f.splits - 1) / f.splits;
+  while (f.splits > 1 && f.per_split * (f.splits - 1) >= kblocks) {   // every CTA of a cluster has work
+    f.splits /= 2;
+    f.per_split = (kblocks + f.splits - 1) / f.splits;
+  }
+  const uint64_t slice = (uint64_t)kFewSlice * (((M + 31) & ~31) + 8) * 4;
+  const uint64_t send = f.splits > 1 ? 8 * slice : kF4EpilogueWarps * kF4StoreBytes;
+  const uint64_t receive = f.splits > 1 ? (uint64_t)(f.splits - 1) * (8 / f.splits) * slice : 0;
+  // A CTA of a cluster holds its tensor memory while it waits for the others, and these wait for theirs without a limit.
+  // What two such CTAs hold (more do not fit on an SM: 320 threads of over 68 registers) must fit together, or two
+  // clusters of two streams could each hold what the other wants. The other kernels of that kind (gemm_few.cuh) hold at
+  // most 128 columns where they leave shared memory for another CTA.
+  f.columns = per_sm == 2 || f.splits > 1 ? 256 : 512;
+  f.scale_at = M <= 64 ? 64 : 128;
+  const int sets = (f.columns - f.scale_at) / (int)kFewScaleSet;
+  f.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - kFewHeader - receive) / stage);
+  if (f.stages > kF4MaxStages) f.stages = kF4MaxStages;
+  if (f.stages > sets) f.stages = sets;
+  if (f.stages > f.per_split) f.stages = f.per_split;
+  uint64_t body = f.stages * stage;
+  if (body < send) body = send;
+  f.recv_at = kFewHeader + body;
+  f.smem = kFewHeader + body + receive;
+  return f;
+}
+
 }  // namespace ab200
 
 using namespace ab200;
 
 extern "C" {
+
+// How a product of M <= 128 tokens runs on `sms` SMs: CTAs of a cluster, columns of tensor memory and bytes of shared
+// memory of each. -2: not by that kernel.
+int ab200_linear_fp4_plan(long long M, int N, int K, int fmt, int sms, int* splits, int* columns, long long* smem) {
+  if (M <= 0 || M > kFewTokens || N <= 0 || K <= 0 || (K % 32) || (N % 8) || fmt < 0 || fmt > 1 || sms <= 0) return -2;
+  const Fp4FewPlan f = fp4_few_plan((int)M, N, K, fmt == kMxfp4, sms);
+  *splits = f.splits;
+  *columns = f.columns;
+  *smem = (long long)f.smem;
+  return 0;
+}
 
 // x: codes [M, K / 2] (rows ldx bytes apart), scale tiles sx [row tiles][k_tiles][512], factors gx fp32 [M] or null;
 // w: codes [groups][N][K / 2] (w_gstride and ldw bytes), scale tiles sw [groups][ceil(N / 128)][k_tiles][512], factors
@@ -982,46 +1044,19 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   };
 
   if (tiles == nullptr && M <= kFewTokens) {
+    const Fp4FewPlan plan = fp4_few_plan((int)M, N, K, mx, sms);
     Fp4FewArgs f;
     memset(&f, 0, sizeof(f));
     f.N = N;
     f.M = (int)M;
     f.kblocks = kblocks;
-    const int x_rows = (int)(M + 15) / 16 * 16;
-    f.b_bytes = (uint32_t)x_rows * 128;
-    const uint64_t stage = kF4ABytes + f.b_bytes + 2ull * step_tiles * kFp4ScaleTile;
-    // More tiles than SMs: two CTAs on each, with half of its shared and tensor memory. Fewer: a tile's steps are
-    // split.
-    const int per_sm = w_row_tiles > sms ? 2 : 1;
-    // (0.31 us a step; the exchange 1.0 to 2.0 us between two CTAs, 1.8 to 3.7 between four, by the tokens: 4096 x 4096,
-    // 1, 64 and 128 tokens 7.2, 7.5, 8.5 us unsplit, 5.7, 6.5, 7.8 with two parts, 5.2, 6.6, 8.4 with four; eight never paid)
-    f.splits = 1;
-    double least = 0.31 * kblocks;
-    for (int parts = 2; parts <= 4 && w_row_tiles * parts <= sms; parts *= 2) {
-      const double t = 0.31 * kblocks / parts + (parts == 2 ? 1.0 + 0.008 * (double)M : 1.8 + 0.015 * (double)M);
-      if (t < least) {
-        least = t;
-        f.splits = parts;
-      }
-    }
-    f.per_split = (kblocks + f.splits - 1) / f.splits;
-    while (f.splits > 1 && f.per_split * (f.splits - 1) >= kblocks) {   // every CTA of a cluster has work
-      f.splits /= 2;
-      f.per_split = (kblocks + f.splits - 1) / f.splits;
-    }
-    const uint64_t slice = (uint64_t)kFewSlice * (((M + 31) & ~31ll) + 8) * 4;
-    const uint64_t send = f.splits > 1 ? 8 * slice : kF4EpilogueWarps * kF4StoreBytes;
-    const uint64_t receive = f.splits > 1 ? (uint64_t)(f.splits - 1) * (8 / f.splits) * slice : 0;
-    f.columns = per_sm == 2 ? 256 : 512;
-    f.scale_at = M <= 64 ? 64 : 128;
-    const int sets = (int)((f.columns - f.scale_at) / kFewScaleSet);
-    f.stages = (int)((227 * 1024 / per_sm - 1024 * (per_sm - 1) - kFewHeader - receive) / stage);
-    if (f.stages > kF4MaxStages) f.stages = kF4MaxStages;
-    if (f.stages > sets) f.stages = sets;
-    if (f.stages > f.per_split) f.stages = f.per_split;
-    uint64_t body = f.stages * stage;
-    if (body < send) body = send;
-    f.recv_at = (uint32_t)(kFewHeader + body);
+    f.splits = plan.splits;
+    f.per_split = plan.per_split;
+    f.stages = plan.stages;
+    f.b_bytes = (uint32_t)plan.x_rows * 128;
+    f.columns = (uint32_t)plan.columns;
+    f.scale_at = (uint32_t)plan.scale_at;
+    f.recv_at = (uint32_t)plan.recv_at;
     f.act = act;
     f.x_scale = reinterpret_cast<const float*>(gx);
     f.w_scale = reinterpret_cast<const float*>(gw);
@@ -1031,10 +1066,10 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
     f.out = reinterpret_cast<bf16*>(out);
     f.ldo = ldo;
     f.status = status;
-    if (!make_maps(x_rows, 1)) return -4;
+    if (!make_maps(plan.x_rows, 1)) return -4;
     auto go = [&](auto kernel) {
       return launch_pdl_cluster(kernel, dim3((unsigned)(w_row_tiles * f.splits)), dim3(kF4Threads),
-                                (size_t)(kFewHeader + body + receive), stream, (unsigned)f.splits, tw, tx, tsw, tsx, f);
+                                (size_t)plan.smem, stream, (unsigned)f.splits, tw, tx, tsw, tsx, f);
     };
     auto by_format = [&](auto nv, auto mxf) { return mx ? go(mxf) : go(nv); };
     const cudaError_t e = plain ? by_format(fp4_few_kernel<false, kF4Plain>, fp4_few_kernel<true, kF4Plain>)

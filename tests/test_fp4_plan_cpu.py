@@ -1,0 +1,45 @@
+"""How the 4-bit products are launched and what the C entries refuse, without a GPU."""
+
+import ctypes
+
+import pytest
+
+from arcticinference_b200 import build
+
+SM_SHARED, CTA_RESERVED = 228 * 1024, 1024
+SMS = 148
+
+
+def _entry(name, *args):
+    fn = getattr(build.load_kernels(), name)
+    fn.restype, fn.argtypes = ctypes.c_int, list(args)
+    return fn
+
+
+def _plan(M, N, K, fmt):
+    P = ctypes.POINTER
+    fn = _entry("ab200_linear_fp4_plan", ctypes.c_longlong, *[ctypes.c_int] * 4, P(ctypes.c_int), P(ctypes.c_int),
+                P(ctypes.c_longlong))
+    parts, columns, smem = ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong()
+    assert fn(M, N, K, fmt, SMS, parts, columns, smem) == 0
+    return parts.value, columns.value, smem.value
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_clusters_that_share_an_sm_both_get_their_tensor_memory(fmt):
+    """CTAs of a cluster wait for one another with their tensor memory in hand, so all that fit on an SM by their shared
+    memory (and there are at most two by their registers) fit into its 512 columns."""
+    seen = set()
+    for M in (1, 5, 16, 17, 32, 33, 64, 65, 100, 128):
+        for N in (8, 128, 264, 520, 1024, 4096, 6144, 9472, 9480, 28672):
+            for K in (32, 256, 1024, 2048, 2304, 4096, 8192, 14336, 32768):
+                parts, columns, smem = _plan(M, N, K, fmt)
+                assert 0 < smem <= 227 * 1024 and columns in (64, 128, 256, 512)
+                assert parts * -(-N // 128) <= SMS or parts == 1
+                if parts > 1:
+                    seen.add(parts)
+                    # (38 KB: the smallest CTA of the bf16 and fp8 clusters, which hold up to 128 columns)
+                    together = min(2, SM_SHARED // (smem + CTA_RESERVED))
+                    assert columns * together <= 512, (M, N, K)
+                    assert columns + 128 <= 512 or smem + 38 * 1024 > SM_SHARED, (M, N, K)
+    assert seen == {2, 4}
