@@ -355,14 +355,14 @@ int ab200_latent_attention(const void* q, long long q_rows, const void* cache, i
 
 // ---- quant_fp4.cu
 int ab200_quant_fp4(const void* x, long long ldx, void* q, long long ldq, void* scale, void* row_scale, long long M,
-                    int K, int fmt, const void* tiles, const void* num_tiles, cudaStream_t stream);
+                    int K, int fmt, const void* tiles, const void* num_tiles, int max_tiles, cudaStream_t stream);
 int ab200_rmsnorm_fp4(const void* x, long long ldx, void* residual, const void* weight, void* q, long long ldq,
                       void* scale, void* row_scale, long long M, int K, float eps, int fmt, cudaStream_t stream);
 int ab200_silu_mul_fp4(const void* x, long long ldx, void* q, long long ldq, void* scale, void* row_scale,
                        long long M, int inter, int nblk, int fmt, cudaStream_t stream);
 int ab200_dequant_fp4(const void* q, long long ldq, const void* scale, const void* row_scale, void* out,
                       long long ldo, long long rows, int K, int group_rows, int fmt, const void* tiles,
-                      const void* num_tiles, cudaStream_t stream);
+                      const void* num_tiles, int max_tiles, cudaStream_t stream);
 
 // ---- gemm_fp4.cu
 int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* gx, const void* w, long long ldw,

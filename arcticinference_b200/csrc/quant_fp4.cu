@@ -54,6 +54,7 @@ struct QuantFp4Args {
   int k_tiles;
   const int4* tiles;    // optional: rows lie in these tiles (group, first row, rows), the scales by tile
   const int* num_tiles;
+  int max_tiles;        // what the list and the scales have room for, whatever *num_tiles says
   int M;
 };
 
@@ -153,7 +154,7 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
 // without rows fills its expert's list up to an even number and begins where the one before it ends.)
 __device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int lane) {
   if (p.tiles == nullptr) return row;
-  const int n = *p.num_tiles, step = (n + 31) / 32;
+  const int n = min(*p.num_tiles, p.max_tiles), step = (n + 31) / 32;
   bool before = false;
   if (lane * step < n) {
     const int4 t = p.tiles[lane * step];
@@ -364,13 +365,13 @@ __global__ void __launch_bounds__(256)
 dequant_fp4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ scale,
                    const float* __restrict__ row_scale, bf16* __restrict__ out, long long ldo, long long rows,
                    int K, int k_tiles, int group_rows, const int4* __restrict__ tiles,
-                   const int* __restrict__ num_tiles) {
+                   const int* __restrict__ num_tiles, int max_tiles) {
   pdl_wait();
   pdl_trigger();
   constexpr int kBlockVecs = MX ? 4 : 2;
   const int nvec = K / 8;
   const int padded = (group_rows + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
-  const long long items = tiles != nullptr ? (long long)*num_tiles * kFp4TileRows : rows;
+  const long long items = tiles != nullptr ? (long long)min(*num_tiles, max_tiles) * kFp4TileRows : rows;
   // (blockIdx.y: a part of the row)
   for (long long item = (long long)blockIdx.x * blockDim.y + threadIdx.y; item < items;
        item += (long long)gridDim.x * blockDim.y) {
@@ -460,11 +461,11 @@ extern "C" {
 
 // x bf16 [M, K], rows ldx apart -> codes [M, K / 2] (rows ldq bytes apart), scale tiles [row tiles][k_tiles][512]
 // with k_tiles = ceil(K / (4 * block)), and for nvfp4 (fmt 0; mxfp4: 1) row_scale fp32 [M]. K: a multiple of 32, at
-// most 32768. With `tiles` (int32 x 4: group, first row, rows; *num_tiles of them, in
+// most 32768. With `tiles` (int32 x 4: group, first row, rows; *num_tiles of them, at most max_tiles, in
 // the order of their rows) a row's scales lie in
 // the row tile of its tile, and rows that no tile holds are left out.
 int ab200_quant_fp4(const void* x, long long ldx, void* q, long long ldq, void* scale, void* row_scale, long long M,
-                    int K, int fmt, const void* tiles, const void* num_tiles, cudaStream_t stream) {
+                    int K, int fmt, const void* tiles, const void* num_tiles, int max_tiles, cudaStream_t stream) {
   if (M <= 0 || K <= 0) return 0;
   if ((K % 32) || K > 32768 || (ldx % 8) || (ldq % 16) || fp4_misaligned(x, q) || fmt < 0 || fmt > 1 ||
       (fmt == kNvfp4 && row_scale == nullptr) || (tiles != nullptr && num_tiles == nullptr))
@@ -480,6 +481,7 @@ int ab200_quant_fp4(const void* x, long long ldx, void* q, long long ldq, void* 
   a.k_tiles = fp4_k_tiles(K, fmt == kMxfp4);
   a.tiles = reinterpret_cast<const int4*>(tiles);
   a.num_tiles = reinterpret_cast<const int*>(num_tiles);
+  a.max_tiles = max_tiles;
   return fmt == kMxfp4 ? launch_quant_fp4<kFp4Plain, true>(a, M, stream)
                        : launch_quant_fp4<kFp4Plain, false>(a, M, stream);
 }
@@ -535,7 +537,7 @@ int ab200_silu_mul_fp4(const void* x, long long ldx, void* q, long long ldq, voi
 // whole of it otherwise); `tiles`: as in ab200_quant_fp4. row_scale null: no factors.
 int ab200_dequant_fp4(const void* q, long long ldq, const void* scale, const void* row_scale, void* out,
                       long long ldo, long long rows, int K, int group_rows, int fmt, const void* tiles,
-                      const void* num_tiles, cudaStream_t stream) {
+                      const void* num_tiles, int max_tiles, cudaStream_t stream) {
   if (rows <= 0 || K <= 0) return 0;
   if ((K % 32) || (ldq % 4) || (ldo % 8) || fp4_misaligned(out, nullptr) || group_rows <= 0 || fmt < 0 || fmt > 1 ||
       (reinterpret_cast<uintptr_t>(q) & 3) || (tiles != nullptr && num_tiles == nullptr))
@@ -549,7 +551,7 @@ int ab200_dequant_fp4(const void* q, long long ldq, const void* scale, const voi
     return launch_pdl(kernel, grid, dim3(across, down), 0, stream, reinterpret_cast<const uint8_t*>(q), ldq,
                       reinterpret_cast<const uint8_t*>(scale), reinterpret_cast<const float*>(row_scale),
                       reinterpret_cast<bf16*>(out), ldo, rows, K, fp4_k_tiles(K, fmt == kMxfp4), group_rows,
-                      reinterpret_cast<const int4*>(tiles), reinterpret_cast<const int*>(num_tiles));
+                      reinterpret_cast<const int4*>(tiles), reinterpret_cast<const int*>(num_tiles), max_tiles);
   };
   const cudaError_t e = fmt == kMxfp4 ? go(dequant_fp4_kernel<true>) : go(dequant_fp4_kernel<false>);
   return e == cudaSuccess ? 0 : -5;

@@ -370,11 +370,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_quant(const at::Tensor& x0, i
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t M = x.size(0), K = x.size(1);
   fp4_width(K, 32768, "quant_fp4");
-  Fp4Out r = fp4_empty(x, M, K, fmt, fp4_tiles(x, tiles, num_tiles));
+  const int64_t row_tiles = fp4_tiles(x, tiles, num_tiles);
+  Fp4Out r = fp4_empty(x, M, K, fmt, row_tiles);
   if (M > 0)
     check(ab200_quant_fp4(x.data_ptr(), x.stride(0), r.q.data_ptr(), K / 2, r.scale.data_ptr(),
                           row_scale_ptr(r.row_scale), M, (int)K, (int)fmt, opt_ptr(tiles), opt_ptr(num_tiles),
-                          stream_of(x)),
+                          (int)row_tiles, stream_of(x)),
           "quant_fp4");
   return {r.q, r.scale, r.row_scale};
 }
@@ -463,7 +464,8 @@ void fp4_dequant_out(const at::Tensor& q, const at::Tensor& scale, const OptTens
   const int64_t R = o.groups * o.rows;
   if (R > 0 && o.K > 0)
     check(ab200_dequant_fp4(q.data_ptr(), q.stride(-2), scale.data_ptr(), opt_ptr(row_scale), out.data_ptr(), o.K, R,
-                            (int)o.K, (int)o.rows, (int)fmt, opt_ptr(tiles), opt_ptr(num_tiles), stream_of(q)),
+                            (int)o.K, (int)o.rows, (int)fmt, opt_ptr(tiles), opt_ptr(num_tiles), (int)row_tiles,
+                            stream_of(q)),
           "dequant_fp4");
 }
 
@@ -543,7 +545,7 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
     g = fmt == 0 ? base + codes + scales : nullptr;
     ldx = K / 2;
     check(ab200_quant_fp4(x.data_ptr(), x.stride(0), base, ldx, base + codes, const_cast<void*>(g), M, (int)K, (int)fmt,
-                          opt_ptr(tiles), opt_ptr(num_tiles), stream),
+                          opt_ptr(tiles), opt_ptr(num_tiles), (int)row_tiles, stream),
           "quant_fp4");
   } else {
     q = xq->data_ptr();

@@ -6,8 +6,9 @@ import torch
 
 from arcticinference_b200 import ops
 from arcticinference_b200.models import quant
+from arcticinference_b200.ops import stream_ops
 
-from fp4_util import FORMATS, oracle_rows, oracle_values, product_bound
+from fp4_util import FORMATS, oracle_rows, oracle_values, product_bound, routing_of
 
 pytestmark = pytest.mark.gpu
 
@@ -31,4 +32,29 @@ def test_clusters_of_two_streams():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(t, want[i]) for t in got[i])
+    ops.check_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_more_tiles_counted_than_listed(fmt):
+    """A count beyond the list: nothing behind the list, or behind the scales that belong to it, is touched."""
+    counts = [100, 0, 60, 129]
+    n, K = sum(counts), 160
+    x = _rand(n, K, seed=1).cuda()
+    w4 = quant.quantize_weight_fp4(_rand(4, 64, K, seed=2, scale=0.1).cuda(), fmt)
+    for even in (False, True):
+        r = routing_of(counts, "cuda", even, slack=0)
+        want = stream_ops.grouped_linear(x, w4, r)
+        for more in (1, 5, 100000):
+            s = routing_of(counts, "cuda", even, slack=0)
+            s.num_tiles += more
+            q = ops.quant_fp4(x, fmt, s)
+            assert torch.equal(q.dequantize(), ops.quant_fp4(x, fmt).dequantize())
+            assert torch.equal(stream_ops.grouped_linear(q, w4, s), want)
+            assert torch.equal(stream_ops.grouped_linear(x, w4, s), want)
+        none = routing_of(counts, "cuda", even, slack=0)
+        none.num_tiles.fill_(-3)
+        out = torch.full((n, K), 7.0, dtype=torch.bfloat16, device="cuda")
+        ops.dequant_fp4(ops.quant_fp4(x, fmt, none), out=out)
+        assert bool((out == 7).all())
     ops.check_status()
