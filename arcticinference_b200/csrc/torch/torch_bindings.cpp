@@ -339,9 +339,11 @@ void on_device_of(const at::Tensor& t, const OptTensor& o) {
   if (has(o)) on_device_of(t, *o);
 }
 
-// Row tiles of a routing: int32 [max_tiles, 4] and how many are in use
+// Row tiles of a routing: int32 [max_tiles, 4] and how many are in use. kNoList: there is no routing (one of no tokens
+// has a list without tiles).
+constexpr int64_t kNoList = -1;
 int64_t fp4_tiles(const at::Tensor& like, const OptTensor& tiles, const OptTensor& num) {
-  if (!has(tiles)) return 0;
+  if (!has(tiles)) return kNoList;
   TORCH_CHECK_VALUE(has(num) && tiles->dim() == 2 && tiles->size(1) == 4 && tiles->scalar_type() == at::kInt &&
                         tiles->is_contiguous() && num->scalar_type() == at::kInt && num->numel() == 1,
                     "a routing's tiles are int32 [n, 4] with their number");
@@ -357,7 +359,7 @@ struct Fp4Out {
 
 Fp4Out fp4_empty(const at::Tensor& x, int64_t M, int64_t K, int64_t fmt, int64_t row_tiles) {
   const auto bytes = x.options().dtype(at::kByte);
-  const int64_t tiles = row_tiles > 0 ? row_tiles : ceil_div(M, kFp4RowTile);
+  const int64_t tiles = row_tiles != kNoList ? row_tiles : ceil_div(M, kFp4RowTile);
   return {at::empty({M, K / 2}, bytes), at::empty({tiles, ceil_div(K, 4 * fp4_block(fmt)), kFp4TileBytes}, bytes),
           at::empty({fmt == 0 ? M : 0}, x.options().dtype(at::kFloat))};
 }
@@ -396,7 +398,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_rmsnorm(const at::Tensor& x0,
                       "rmsnorm_fp4: a contiguous bf16 residual ", x.sizes());
     on_device_of(x, residual);
   }
-  Fp4Out r = fp4_empty(x, M, K, fmt, 0);
+  Fp4Out r = fp4_empty(x, M, K, fmt, kNoList);
   if (M > 0)
     check(ab200_rmsnorm_fp4(x.data_ptr(), x.stride(0), const_cast<void*>(opt_ptr(residual)), weight.data_ptr(),
                             r.q.data_ptr(), K / 2, r.scale.data_ptr(), row_scale_ptr(r.row_scale), M, (int)K,
@@ -413,7 +415,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fp4_silu_mul(const at::Tensor& x0
   const int64_t M = x.size(0), K = x.size(1) / 2, inter = K / nblk;
   fp4_width(K, 32768, "silu_mul_fp4");
   TORCH_CHECK_VALUE(inter % 8 == 0, "silu_mul_fp4: blocks of a multiple of 8 columns, got ", inter);
-  Fp4Out r = fp4_empty(x, M, K, fmt, 0);
+  Fp4Out r = fp4_empty(x, M, K, fmt, kNoList);
   if (M > 0)
     check(ab200_silu_mul_fp4(x.data_ptr(), x.stride(0), r.q.data_ptr(), K / 2, r.scale.data_ptr(),
                              row_scale_ptr(r.row_scale), M, (int)inter, (int)nblk, (int)fmt, stream_of(x)),
@@ -437,7 +439,7 @@ Fp4Operand fp4_operand(const at::Tensor& q, const at::Tensor& scale, const OptTe
   TORCH_CHECK_VALUE(scale.scalar_type() == at::kByte && scale.is_contiguous() && aligned(scale, 16) &&
                         scale.dim() == q.dim() + 1 && scale.size(-1) == kFp4TileBytes &&
                         scale.size(-2) == ceil_div(o.K, 4 * fp4_block(fmt)) &&
-                        scale.size(-3) == (row_tiles > 0 ? row_tiles : ceil_div(o.rows, kFp4RowTile)) &&
+                        scale.size(-3) == (row_tiles != kNoList ? row_tiles : ceil_div(o.rows, kFp4RowTile)) &&
                         (q.dim() == 2 || scale.size(0) == o.groups),
                     what, ": scale tiles ", scale.sizes(), " do not belong to codes ", q.sizes());
   on_device_of(q, scale);
@@ -486,7 +488,7 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
                  const OptTensor& tiles, const OptTensor& num_tiles, bool even, at::Tensor& out,
                  const at::Tensor& status) {
   const int64_t row_tiles = fp4_tiles(wq, tiles, num_tiles);
-  const Fp4Operand w = fp4_operand(wq, ws, wg, fmt, 0, "4-bit weight");
+  const Fp4Operand w = fp4_operand(wq, ws, wg, fmt, kNoList, "4-bit weight");
   const c10::cuda::CUDAGuard guard(wq.device());
   const cudaStream_t stream = stream_of(wq);
   const int64_t N = w.rows, K = w.K;
@@ -511,7 +513,7 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
   TORCH_CHECK_VALUE(status.scalar_type() == at::kInt && status.is_contiguous() && status.numel() >= 8,
                     "4-bit product: status is int32 [8]");
   on_device_of(wq, status);
-  const bool grouped = row_tiles > 0;
+  const bool grouped = row_tiles != kNoList;
   TORCH_CHECK_VALUE(grouped == (wq.dim() == 3), "4-bit product: several matrices go with a routing");
   TORCH_CHECK_VALUE(N % (gate ? 32 : 8) == 0, "4-bit product: N a multiple of ", gate ? 32 : 8, ", got ", N);
   const int64_t width = gate ? N / 2 : N;

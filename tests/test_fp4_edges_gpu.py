@@ -58,3 +58,22 @@ def test_more_tiles_counted_than_listed(fmt):
         ops.dequant_fp4(ops.quant_fp4(x, fmt, none), out=out)
         assert bool((out == 7).all())
     ops.check_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_routing_of_no_tokens(fmt):
+    """Its list has no tiles: results without rows, as from the bf16 products."""
+    E, N, K = 4, 64, 96
+    w = _rand(E, N, K, seed=1, scale=0.1).cuda()
+    w4 = quant.quantize_weight_fp4(w, fmt)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    r = stream_ops.Routing(None, None, None, 1, E, torch.empty(0, 4, **i32), torch.zeros(1, **i32), counts=[0] * E)
+    x = torch.empty(0, K, dtype=torch.bfloat16, device="cuda")
+    for act, width in ((None, N), ("silu", N // 2)):
+        got = stream_ops.grouped_linear(x, w4, r, act)
+        assert got.shape == (0, width) == stream_ops.grouped_linear(x, w, r, act).shape
+        q = ops.quant_fp4(x, fmt, r)
+        assert stream_ops.grouped_linear(q, w4, r, act).shape == (0, width) and q.dequantize().shape == (0, K)
+    with pytest.raises(ValueError):
+        stream_ops.grouped_linear(torch.empty(0, K + 32, dtype=torch.bfloat16, device="cuda"), w4, r)
+    ops.check_status()
