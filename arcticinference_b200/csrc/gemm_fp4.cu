@@ -979,7 +979,7 @@ int ab200_linear_fp4_plan(long long M, int N, int K, int fmt, int sms, int* spli
 // w: codes [groups][N][K / 2] (w_gstride and ldw bytes), scale tiles sw [groups][ceil(N / 128)][k_tiles][512], factors
 // gw fp32 [groups][N] or null; out bf16. K a multiple of 32, N of 8 (of 32 with a gate), strides of codes multiples of
 // 16 bytes, ldo and ldr of 8 elements. fmt: 0 nvfp4, 1 mxfp4. act: 0, 1 (GELU); gate: 0, 1 (silu), 2 (gelu_tanh), 3
-// (clamped swish): rows of w alternate 16 gate and 16 up rows and out has N / 2 columns. With `tiles` (int32 x 4:
+// (clamped swish): rows of w alternate 16 gate and 16 up rows and out has N / 2 columns; only with `tiles`. With `tiles` (int32 x 4:
 // group, first row, rows; *num_tiles of them, at most max_tiles) row tile i's scales are sx's i-th row tile; even: every
 // group has an even number of tiles, all but the last two full, of which the last may be empty.
 int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* gx, const void* w, long long ldw,
@@ -992,7 +992,7 @@ int ab200_linear_fp4(const void* x, long long ldx, const void* sx, const void* g
   if ((K % 32) || (N % 8) || (gate != 0 && N % 32) || gate < 0 || gate > 3 || act < 0 || act > 1 || fmt < 0 || fmt > 1 ||
       (ldx % 16) || (ldw % 16) || (w_gstride % 16) || (ldo % 8) || (ldr % 8) || odd(x, 15) || odd(w, 15) ||
       odd(sx, 15) || odd(sw, 15) || odd(out, 15) || odd(residual, 15) || M > 0x7fffff00ll ||
-      (gate != 0 && (act != 0 || bias != nullptr || residual != nullptr)) ||
+      (gate != 0 && (tiles == nullptr || act != 0 || bias != nullptr || residual != nullptr)) ||
       (tiles == nullptr ? groups != 1 : num_tiles == nullptr || bias != nullptr || residual != nullptr))
     return -2;
   const bool mx = fmt == kMxfp4;

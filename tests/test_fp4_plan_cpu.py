@@ -43,3 +43,20 @@ def test_clusters_that_share_an_sm_both_get_their_tensor_memory(fmt):
                     assert columns * together <= 512, (M, N, K)
                     assert columns + 128 <= 512 or smem + 38 * 1024 > SM_SHARED, (M, N, K)
     assert seen == {2, 4}
+
+
+def _linear_fp4(M, N, K, gate, act=0, tiles=False):
+    """The C entry's answer to a call with pointers that nothing reads before the checks are done."""
+    P, L, I, F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
+    fn = _entry("ab200_linear_fp4", P, L, P, P, P, L, L, P, P, P, L, L, I, I, I, I, P, P, L, I, I, F, F, P, P, I, I, P, P)
+    room = ctypes.create_string_buffer(4096)
+    at = ctypes.addressof(room) + 255 & ~255
+    return fn(at, K // 2, at, None, at, K // 2, 0, at, None, at, N, M, N, K, 1, 0, None, None, 0, act, gate, 0.0, 0.0,
+              at if tiles else None, at if tiles else None, 0, 0, at, None)
+
+
+@pytest.mark.parametrize("M", [1, 100, 129, 300, 5000])
+@pytest.mark.parametrize("gate", [1, 2, 3])
+def test_a_gate_without_a_list_is_refused(M, gate):
+    """Only products of lists join gate and up: others would store N columns where out has N / 2."""
+    assert _linear_fp4(M, 256, 512, gate) == -2
