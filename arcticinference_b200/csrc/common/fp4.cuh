@@ -89,6 +89,11 @@ __device__ __forceinline__ void tmem_ld_frag_x4(uint32_t taddr, uint32_t (&r)[16
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // Transposed 8 x 8 matrices of 16-bit numbers between registers and shared memory; lane l gives the address of row
 // l % 8 of matrix l / 8.
 __device__ __forceinline__ void stmatrix_t4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

@@ -137,7 +137,37 @@ __device__ __forceinline__ uint32_t f4_piece(int token, int piece) {
 
 // The factor of token c of a tile
 __device__ __forceinline__ float f4_token(const float* x_scale, int row0, int c, int nrows) {
-  return x_scale == nullptr ? 1.f : c < nrows ? x_scale[row0 + c] : 0.f;
+  return x_scale == nullptr || c >= nrows ? 1.f : x_scale[row0 + c];
+}
+
+// Whether a factor lies outside of 2^-63 .. 2^63 (or is none). The others are multiplied with each other first, which stays
+// within 2^-126 .. 2^126: one operation less per number than a sum times both.
+__device__ __forceinline__ bool f4_far(float factor) {
+  return (__float_as_uint(factor) & 0x7fffffffu) - 0x20000000u > 0x3f000000u;
+}
+// v g h for any factors (rows near 2^-126 or 2^127, whose factor and a feature's may have a product outside of fp32): a sum of
+// at least 1 takes the smaller factor first, one below 1 the larger, so that what overflows or vanishes on the way does so
+// in the end.
+__device__ __forceinline__ float f4_scaled(float v, float g, float h) {
+  const bool swap = fabsf(g) > fabsf(h);
+  const float less = swap ? h : g, more = swap ? g : h;
+  return fabsf(v) < 1.f ? v * more * less : v * less * more;
+}
+// Every other 32 tokens of a warp's 32 features, from `first` on, multiplied by both factors where they lie in tensor memory
+// (rare, and small: the epilogues have to stay in the instruction cache)
+__device__ __noinline__ void f4_rescale(uint32_t t_addr, int first, int row0, int nrows, const float* x_scale, float h) {
+  __syncwarp();
+#pragma unroll 1
+  for (int c = first; c < nrows; c += (c & 24) == 24 ? 40 : 8) {
+    uint32_t r[8];
+    tmem_ld_x8(t_addr + (uint32_t)c, r);
+    tmem_ld_wait_dep(r);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      r[t] = __float_as_uint(f4_scaled(__uint_as_float(r[t]), f4_token(x_scale, row0, c + t, nrows), h));
+    tmem_st_x8(t_addr + (uint32_t)c, r);
+  }
+  tmem_st_wait();
 }
 
 // 16 gate rows (lo) and the 16 up rows they belong to (hi), joined into the staging tile
@@ -502,17 +532,28 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     Factors coming_factors = fetch(coming);
     for (int w = first_work; w < total_work; w += work_step) {
       const F4Work t = coming;
-      const Factors fc = coming_factors;
+      Factors fc = coming_factors;
       coming = work(w + work_step);
       if (t.nrows <= 0) {
         coming_factors = fetch(coming);
         continue;
       }
       const int feature0 = (kCtas * t.nt + rank) * 128 + quad * 32;
+      bool far = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) far |= f4_far(fc.ft.h[i]) | (PAIR || i < 2 ? f4_far(fc.gx[i]) : false);
+      far = __any_sync(0xffffffffu, far);
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, 1700 + acc, w)))
         break;
       tc_fence_after();
       const uint32_t t_addr = tmem_base + f4_accumulator(acc, t.nrows) + ((uint32_t)(quad * 32) << 16);
+      if (__builtin_expect(far, 0)) {
+        const int f = min(feature0 + lane, p.N - 1);
+        f4_rescale(t_addr, 32 * half, t.row0, t.nrows, p.x_scale,
+                   p.w_scale != nullptr ? p.w_scale[(long long)t.group * p.N + f] : 1.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fc.ft.h[i] = fc.gx[i] = 1.f;
+      }
       if (!PAIR) {
         // (half the registers: 32 tokens at a time)
         coming_factors = fetch(coming);
@@ -777,9 +818,21 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
       float gx = f4_token(p.x_scale, 0, 32 * half + lane, p.M);
       ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.status, 1900, n));
       tc_fence_after();
+      const float* x_scale = p.x_scale;
+      bool far = f4_far(gx) | f4_far(f4_token(x_scale, 0, 32 * half + 64 + lane, p.M));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) far |= f4_far(ft.h[i]);
+      if (ok && __any_sync(0xffffffffu, far)) {
+        const int f = min(feature0 + lane, p.N - 1);
+        f4_rescale(t_addr, 32 * half, 0, p.M, x_scale, p.w_scale != nullptr ? p.w_scale[f] : 1.f);
+        x_scale = nullptr;
+        gx = 1.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ft.h[i] = 1.f;
+      }
       if (ok && feature0 < p.N)
         for (int c0 = 32 * half; c0 < p.M; c0 += 64) {
-          const float next = f4_token(p.x_scale, 0, c0 + 64 + lane, p.M);
+          const float next = f4_token(x_scale, 0, c0 + 64 + lane, p.M);
           uint32_t lo[16], hi[16];
           __syncwarp();
           tmem_ld_frag_x4(t_addr + (uint32_t)c0, lo);
@@ -857,6 +910,9 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     __syncwarp();
     cluster_arrive();   // (nobody leaves before its sums have been received)
     if (mine_too && ok) {
+      bool far = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) far |= f4_far(h[e]);
       const float* own = reinterpret_cast<const float*>(ring + my * source_bytes) + (size_t)(8 * part) * pitch;
       const float* others = reinterpret_cast<const float*>(smem + p.recv_at) + (size_t)(8 * part) * pitch;
       for (int m = first; m < p.M; m += across) {
@@ -875,9 +931,15 @@ fp4_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] += a[e * pitch];
         }
+        if (far || f4_far(gx)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = f4_scaled(v[e], gx, h[e]) + bias[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = v[e] * (gx * h[e]) + bias[e];
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = v[e] * (gx * h[e]) + bias[e];
           if (EPI == kF4Any && p.act == 1) v[e] = gelu_exact(v[e]);
         }
         if (EPI == kF4Any && p.residual != nullptr) {

@@ -77,3 +77,77 @@ def test_a_routing_of_no_tokens(fmt):
     with pytest.raises(ValueError):
         stream_ops.grouped_linear(torch.empty(0, K + 32, dtype=torch.bfloat16, device="cuda"), w4, r)
     ops.check_status()
+
+
+def _relative_bound(x, w, y):
+    """As product_bound, without the absolute term that it allows: half a bf16 step (2^-134 among the smallest numbers), fp32
+    sums, the roundings of two factors."""
+    mag = x.abs() @ w.abs().t()
+    return (2.0 ** -8 + 2.0 ** -22) * y.abs() + (x.shape[1] / 16 + 8) * 2.0 ** -23 * mag + 2.0 ** -134
+
+
+@pytest.mark.parametrize("M,K", [(1, 512), (20, 512), (5, 4096), (128, 4096), (150, 512), (300, 512)])
+def test_factors_whose_product_leaves_the_range(M, K):
+    """Factors of rows and features whose product fp32 does not hold, though that with the sum is an ordinary number."""
+    fmt, N = "nvfp4", 264
+    x, w = _rand(M, K, seed=1).abs(), _rand(N, K, seed=2).abs()
+    x = (x.float() * 2.0 ** -100).to(torch.bfloat16)
+    w = (w.float() * 2.0 ** -32).to(torch.bfloat16)
+    w[1::3] = (w[1::3].float() * 2.0 ** 31).to(torch.bfloat16)           # beside ordinary features
+    x[::2] = (x[::2].float() * 2.0 ** 99).to(torch.bfloat16)             # and ordinary rows
+    w4 = quant.quantize_weight_fp4(w.cuda(), fmt)
+    g, h = ops.quant_fp4(x.cuda(), fmt).row_scale, w4.row_scale
+    assert M == 1 or float(g.min() * h.min()) == 0          # (2^-150 or less: half the smallest number)
+    res, bias = torch.zeros(M, N, dtype=torch.bfloat16), torch.zeros(N, dtype=torch.bfloat16)
+    xd, wd = oracle_rows(x, fmt).cuda(), oracle_values(w4.q, w4.scale, w4.row_scale, fmt).cuda()
+    y = xd @ wd.t()
+    assert float(y.min()) > 2.0 ** -126
+    for kw in ({}, {"residual": res.cuda()}, {"bias": bias.cuda()}):
+        got = ops.linear(x.cuda(), w4, **kw)
+        bad = (got.double() - y).abs() > _relative_bound(xd, wd, y)
+        assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist(), got[bad][0], y[bad][0])
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M,K", [(20, 512), (5, 4096), (150, 512), (300, 512)])
+def test_sums_of_zero_beside_the_largest_factors(M, K):
+    fmt, N = "nvfp4", 136
+    x, w = torch.zeros(M, K, dtype=torch.bfloat16), torch.zeros(N, K, dtype=torch.bfloat16)
+    x[:, 0], w[:, K - 1] = 2.0 ** 120, 2.0 ** 60
+    x[:, 100], w[:, 100] = 1e-6, 1e-6          # (its code and scale are zero beside such numbers)
+    w4 = quant.quantize_weight_fp4(w.cuda(), fmt)
+    assert bool((ops.linear(x.cuda(), w4) == 0).all())
+    assert bool((ops.linear(x.cuda(), w4, residual=torch.ones(M, N, dtype=torch.bfloat16, device="cuda")) == 1).all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("even", [False, True])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_experts_factors_whose_product_leaves_the_range(even, act):
+    """Gate and up of ordinary size, reached through factors far from 1 on both sides."""
+    fmt, N, K, counts = "nvfp4", 64, 256, [140, 0, 300, 7]
+    n = sum(counts)
+    x, w = _rand(n, K, seed=1).abs(), _rand(4, N, K, seed=2, scale=0.01).abs()
+    small, large = (x.float() * 2.0 ** -110).to(torch.bfloat16), (w.float() * 2.0 ** 110).to(torch.bfloat16)
+    tiny, little = (x.float() * 2.0 ** -100).to(torch.bfloat16), (w.float() * 2.0 ** -20).to(torch.bfloat16)
+    for a, b in ((small, large), (tiny, little)):
+        w4 = quant.quantize_weight_fp4(b.cuda(), fmt)
+        got = stream_ops.grouped_linear(a.cuda(), w4, routing_of(counts, "cuda", even), act)
+        first = 0
+        for e, c in enumerate(counts):
+            if c:
+                xd = oracle_rows(a[first:first + c], fmt).cuda()
+                wd = oracle_values(w4.q[e], w4.scale[e], w4.row_scale[e], fmt).cuda()
+                y = xd @ wd.t()
+                bound = _relative_bound(xd, wd, y)
+                if act is not None:
+                    g, u = (t.reshape(c, N // 2) for t in y.reshape(c, N // 32, 2, 16).unbind(2))
+                    eg, eu = (t.reshape(c, N // 2) for t in
+                              (bound - 2.0 ** -8 * y).reshape(c, N // 32, 2, 16).unbind(2))
+                    y = g * torch.sigmoid(g) * u
+                    # |d silu| < 1.1; exponential and division 2^-20 of the result; g, u >= 0
+                    bound = 2.0 ** -8 * y + 1.1 * u * eg + g * eu + 2.0 ** -20 * y + 2.0 ** -134
+                bad = (got[first:first + c].double() - y).abs() > bound
+                assert not bad.any(), (e, int(bad.sum()), bad.nonzero()[0].tolist(), got[first:first + c][bad][0], y[bad][0])
+            first += c
+    ops.check_status()
