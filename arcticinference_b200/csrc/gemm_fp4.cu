@@ -140,10 +140,11 @@ __device__ __forceinline__ float f4_token(const float* x_scale, int row0, int c,
   return x_scale == nullptr || c >= nrows ? 1.f : x_scale[row0 + c];
 }
 
-// Whether a factor lies outside of 2^-63 .. 2^63 (or is none). The others are multiplied with each other first, which stays
-// within 2^-126 .. 2^126: one operation less per number than a sum times both.
+// Whether a factor lies outside of 2^-63 .. 2^63. The others are multiplied with each other first, which stays within
+// 2^-126 .. 2^126: one operation less per number than a sum times both. (A factor that is no number gives none either way,
+// and should not move its neighbours, whose bias is added to an unrounded product, to the other.)
 __device__ __forceinline__ bool f4_far(float factor) {
-  return (__float_as_uint(factor) & 0x7fffffffu) - 0x20000000u > 0x3f000000u;
+  return (__float_as_uint(factor) & 0x7fffffffu) - 0x20000000u > 0x3f000000u && factor == factor;
 }
 // v g h for any factors (rows near 2^-126 or 2^127, whose factor and a feature's may have a product outside of fp32): a sum of
 // at least 1 takes the smaller factor first, one below 1 the larger, so that what overflows or vanishes on the way does so

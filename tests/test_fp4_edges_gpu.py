@@ -151,3 +151,18 @@ def test_experts_factors_whose_product_leaves_the_range(even, act):
                 assert not bad.any(), (e, int(bad.sum()), bad.nonzero()[0].tolist(), got[first:first + c][bad][0], y[bad][0])
             first += c
     ops.check_status()
+
+
+@pytest.mark.parametrize("M,K", [(20, 512), (100, 4096), (300, 512)])
+def test_rows_that_are_no_numbers_move_no_bit_of_others(M, K):
+    N = 264
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=0.1).cuda(), "nvfp4")
+    g = (0.01 + torch.rand(N, generator=torch.Generator().manual_seed(3))).cuda()
+    w4 = quant.Fp4Weight(w4.q, w4.scale, g, "nvfp4")
+    x, bias = _rand(M, K, seed=2), _rand(N, seed=4, scale=10.0).cuda()
+    clean = ops.linear(x.cuda(), w4, bias=bias)
+    x[3, 7], x[M - 1, 200] = float("inf"), float("nan")
+    got = ops.linear(x.cuda(), w4, bias=bias)
+    assert got[[3, M - 1]].isnan().all()
+    keep = [i for i in range(M) if i not in (3, M - 1)]
+    assert torch.equal(got[keep], clean[keep])
