@@ -59,6 +59,10 @@ def _bf16_matrix(x, what: str) -> None:
     _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == torch.bfloat16, "%s: a bf16 matrix", what)
 
 
+def _width(K: int, most: int, what: str) -> None:
+    _need(K % 32 == 0 and 0 < K <= most, "%s: a multiple of 32 columns up to %d, got %d", what, most, K)
+
+
 def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", routing=None):
     """bf16 rows [M, K], K a multiple of 32 and at most 32768 -> ``Fp4Rows``. ``routing`` (a ``stream_ops.Routing``): the
     rows are sorted by expert and lie in its tiles; rows that no tile holds are left out."""
@@ -66,8 +70,7 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", routing=None):
     if not x.is_cuda:
         from ..models import quant
         _bf16_matrix(x, "quant_fp4")
-        K = x.shape[1]
-        _need(K % 32 == 0 and 0 < K <= 32768, "quant_fp4: K a multiple of 32 up to 32768, got %d", K)
+        _width(x.shape[1], 32768, "quant_fp4")
         r = quant.quantize_fp4_ref(x, fmt)
         return r if routing is None else quant.Fp4Rows(r.q, r.scale, r.row_scale, fmt, routing)
     o = _ops()
@@ -99,6 +102,11 @@ def rmsnorm_fp4(x: torch.Tensor, weight: torch.Tensor, eps: float, residual=None
     code = _code(fmt)
     if not x.is_cuda:
         from ..models import quant
+        _bf16_matrix(x, "rmsnorm_fp4")
+        _width(x.shape[1], 16384, "rmsnorm_fp4")
+        for name, t, shape in (("weight", weight, x.shape[1:]), ("residual", residual, x.shape)):
+            _need(t is None or t.dtype == torch.bfloat16 and t.shape == shape and t.is_contiguous(),
+                  "rmsnorm_fp4: a contiguous bf16 %s %s", name, tuple(shape))
         return quant.quantize_fp4_ref(ref.rmsnorm(x, weight, eps, residual), fmt)
     o = _ops()
     q, scale, g = o.rmsnorm(x, weight, eps, residual, code)
@@ -111,8 +119,12 @@ def silu_mul_fp4(x: torch.Tensor, nblk: int = 1, fmt: str = "nvfp4"):
     code = _code(fmt)
     if not x.is_cuda:
         from ..models import quant
-        _need(x.dim() == 2 and nblk >= 1 and x.shape[1] % (2 * nblk) == 0, "silu_mul_fp4: %s in %d (gate | up) blocks",
+        _bf16_matrix(x, "silu_mul_fp4")
+        _need(nblk >= 1 and x.shape[1] % (2 * nblk) == 0, "silu_mul_fp4: %s in %d (gate | up) blocks",
               tuple(x.shape), nblk)
+        K = x.shape[1] // 2
+        _width(K, 32768, "silu_mul_fp4")
+        _need(K // nblk % 8 == 0, "silu_mul_fp4: blocks of a multiple of 8 columns, got %d", K // nblk)
         return quant.quantize_fp4_ref(ref.silu_mul_blocked(x, nblk), fmt)
     o = _ops()
     q, scale, g = o.silu_mul(x, nblk, code)

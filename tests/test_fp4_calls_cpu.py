@@ -7,6 +7,7 @@ from arcticinference_b200 import ops
 from arcticinference_b200.models import quant
 from arcticinference_b200.ops import stream_ops
 
+import fp4_calls
 from fp4_util import FORMATS, routing_of
 
 
@@ -21,3 +22,21 @@ def test_a_routing_of_no_tokens(fmt):
     x = torch.empty(0, 96, dtype=torch.bfloat16)
     assert stream_ops.grouped_linear(x, w4, r).shape == (0, 64)
     assert stream_ops.grouped_linear(ops.quant_fp4(x, fmt, r), w4, r, "silu").shape == (0, 32)
+
+
+def _all_refused(calls):
+    taken = {}
+    for name, f in calls.items():
+        try:
+            f()
+            taken[name] = "not refused"
+        except ValueError:
+            pass
+        except Exception as e:          # noqa: BLE001 (which one is the answer)
+            taken[name] = repr(e)[:90]
+    assert not taken, taken
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_refused_norms_and_activations(fmt):
+    _all_refused(fp4_calls.norm_and_activation("cpu", fmt))

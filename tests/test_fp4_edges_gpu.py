@@ -8,6 +8,7 @@ from arcticinference_b200 import ops
 from arcticinference_b200.models import quant
 from arcticinference_b200.ops import stream_ops
 
+import fp4_calls
 from fp4_util import FORMATS, oracle_rows, oracle_values, product_bound, routing_of
 
 pytestmark = pytest.mark.gpu
@@ -166,3 +167,17 @@ def test_rows_that_are_no_numbers_move_no_bit_of_others(M, K):
     assert got[[3, M - 1]].isnan().all()
     keep = [i for i in range(M) if i not in (3, M - 1)]
     assert torch.equal(got[keep], clean[keep])
+
+
+def _all_refused(calls):
+    for name, f in calls.items():
+        with pytest.raises(ValueError):
+            f()
+            raise AssertionError("not refused: " + name)
+    torch.cuda.synchronize()
+    ops.check_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_refused_norms_and_activations(fmt):
+    _all_refused(fp4_calls.norm_and_activation("cuda", fmt))
