@@ -85,6 +85,8 @@ def dequant_fp4(rows, out: torch.Tensor = None) -> torch.Tensor:
     if not rows.is_cuda:
         from ..models import quant
         plain = rows if rows.routing is None else quant.Fp4Rows(rows.q, rows.scale, rows.row_scale, rows.fmt)
+        _need(out is None or out.dtype == torch.bfloat16 and out.shape == rows.shape and out.is_contiguous(),
+              "dequant_fp4: out is a contiguous bf16 tensor of the rows' shape")
         y = quant.dequantize_fp4_ref(plain).to(torch.bfloat16)
         return y if out is None else out.copy_(y)
     r, o = rows.routing, _ops()
@@ -165,18 +167,49 @@ def linear_fp4(x, w, bias=None, residual=None, act=None, out=None) -> torch.Tens
     return out
 
 
+def _lies(t, ok: bool, what: str) -> None:
+    """What the kernels' 16-byte accesses need of a CPU tensor too."""
+    _need(t.device.type == "cpu", "4-bit product: %s on %s beside tensors on the CPU", what, t.device)
+    _need(ok, "4-bit product: %s: rows on 16-byte boundaries", what)
+
+
+def _ref_operand(t, what: str) -> None:
+    """Codes, scales and factors as the kernels read them."""
+    _lies(t.q, t.q.stride(-1) == 1 and all(s % 16 == 0 for s in t.q.stride()[:-1]) and t.q.data_ptr() % 16 == 0, what)
+    _lies(t.scale, t.scale.is_contiguous(), what + "' scales")
+    if t.row_scale is not None:
+        _lies(t.row_scale, t.row_scale.is_contiguous(), what + "' factors")
+
+
+def _ref_rows(x, w, routing=None):
+    """The numbers that the rows of a product stand for, fp32."""
+    from ..models import quant
+    K = w.shape[-1]
+    _need(K > 0, "4-bit product: rows without columns")
+    _need(len(x.shape) == 2 and x.shape[1] == K, "4-bit product: rows %s and weight %s", tuple(x.shape), tuple(w.shape))
+    _ref_operand(w, "weight")
+    rows = x
+    x, q, scale, g = _operand(x, w, routing)
+    if x is None:
+        _ref_operand(rows, "rows")
+        return quant.dequantize_fp4_ref(quant.Fp4Rows(q, scale, g, w.fmt))
+    _lies(x, True, "rows")
+    return quant.dequantize_fp4_ref(quant_fp4(x, w.fmt))
+
+
 def _linear_ref(x, w, bias, residual, act, out):
     from ..models import quant
-    N, K = w.shape
-    _need(K > 0, "linear_fp4: rows without columns")
-    _need(len(x.shape) == 2 and x.shape[1] == K, "linear_fp4: rows %s and weight %s", tuple(x.shape), (N, K))
-    M = x.shape[0]
+    N = w.shape[0]
+    v = _ref_rows(x, w)
+    M = v.shape[0]
+    _need(N % 8 == 0, "4-bit product: N a multiple of 8, got %d", N)
     for name, t, shape in (("bias", bias, (N,)), ("residual", residual, (M, N)), ("out", out, (M, N))):
-        _need(t is None or t.dtype == torch.bfloat16 and tuple(t.shape) == shape, "linear_fp4: %s is bf16 %s", name,
-              shape)
-    x, q, scale, g = _operand(x, w)
-    rows = quant.Fp4Rows(q, scale, g, w.fmt) if x is None else quant_fp4(x, w.fmt)
-    y = quant.dequantize_fp4_ref(rows) @ quant.dequantize_fp4_ref(w).t()
+        if t is not None:
+            _need(t.dtype == torch.bfloat16 and tuple(t.shape) == shape, "linear_fp4: %s is bf16 %s", name, shape)
+            _lies(t, t.is_contiguous() if name == "bias" else
+                  t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0, name)
+    _need(out is None or M <= 1 or out.stride(0) >= N, "4-bit product: rows of out overlap")
+    y = v @ quant.dequantize_fp4_ref(w).t()
     if bias is not None:
         y = y + bias.float()
     if act == "gelu":
@@ -195,10 +228,10 @@ def grouped_linear_fp4(x, w, routing, act=None) -> torch.Tensor:
     act = None if act is None else stream_ops.Gate.of(act)
     wq = getattr(w, "q", None)
     _need(wq is not None and wq.dim() == 3 and hasattr(w, "fmt"), "grouped_linear_fp4: an Fp4Weight [E, N, K]")
-    if not wq.is_cuda:
-        return _grouped_ref(x, w, routing, act)
     _need(routing.num_experts == wq.shape[0], "grouped_linear_fp4: a routing of %d experts and %d matrices",
           routing.num_experts, wq.shape[0])
+    if not wq.is_cuda:
+        return _grouped_ref(x, w, routing, act)
     x, xq, xs, xg = _operand(x, w, routing)
     o = _ops()
     launch_counter.add(1 if x is None else 2)
@@ -208,13 +241,11 @@ def grouped_linear_fp4(x, w, routing, act=None) -> torch.Tensor:
 
 def _grouped_ref(x, w, routing, act):
     from ..models import quant
-    E, N, K = w.shape
-    _need(len(x.shape) == 2 and x.shape[1] == K, "grouped_linear_fp4: rows %s and weights %s", tuple(x.shape), (E, N, K))
+    N = w.shape[1]
+    v = _ref_rows(x, w, routing)
     _need(N % (32 if act else 8) == 0, "grouped_linear_fp4: N a multiple of %d, got %d", 32 if act else 8, N)
-    x, q, scale, g = _operand(x, w, routing)
-    x = quant.dequantize_fp4_ref(quant.Fp4Rows(q, scale, g, w.fmt) if x is None else quant_fp4(x, w.fmt))
     m = quant.dequantize_fp4_ref(w)
-    y = torch.cat([xe @ m[e].t() for e, xe in enumerate(x.split(routing.counts))])
+    y = torch.cat([ve @ m[e].t() for e, ve in enumerate(v.split(routing.counts))])
     if act is not None:
         v = y.reshape(y.shape[0], N // 32, 2, 16)
         y = act.join(v[:, :, 0], v[:, :, 1]).reshape(y.shape[0], N // 2)

@@ -4,6 +4,7 @@ import torch
 
 from arcticinference_b200 import ops
 from arcticinference_b200.models import quant
+from arcticinference_b200.ops import stream_ops
 
 from fp4_util import routing_of
 
@@ -32,4 +33,54 @@ def norm_and_activation(device, fmt):
         "activation: no blocks": lambda: ops.silu_mul_blocked(r(4, 64), 0, quant=fmt),
         "activation: fp32 rows": lambda: ops.silu_mul_blocked(r(4, 128).float(), quant=fmt),
         "activation: three dimensions": lambda: ops.silu_mul_blocked(r(2, 2, 128), quant=fmt),
+    }
+
+
+def products(device, fmt):
+    r = lambda *s: _rand(*s, device=device)
+    w = lambda *s: quant.quantize_weight_fp4(r(*s), fmt)
+    other = {"nvfp4": "mxfp4", "mxfp4": "nvfp4"}[fmt]
+    x, w4, e4, list2 = r(4, 64), w(40, 64), w(2, 32, 64), routing_of([2, 2], device)
+    q = ops.quant_fp4(x, fmt)
+    lone, buf = r(1, 40), r(4, 48)
+    scaled = quant.Fp4Weight(w4.q, w4.scale, torch.ones(80, device=device)[::2], fmt)
+    apart = torch.zeros(2 * q.scale.numel(), dtype=torch.uint8, device=device).view(*q.scale.shape, 2)[..., 0]
+    codes = torch.zeros(4, 40, dtype=torch.uint8, device=device)
+    return {
+        "36 features": lambda: ops.linear(x, w(36, 64)),
+        "fp32 rows": lambda: ops.linear(x.float(), w4),
+        "three dimensions": lambda: ops.linear(x[None], w4),
+        "another width": lambda: ops.linear(r(4, 96), w4),
+        "rows of the other format": lambda: ops.linear(ops.quant_fp4(x, other), w4),
+        "rows above 32768": lambda: ops.linear(r(1, 32800), quant.Fp4Weight(
+            torch.zeros(8, 16400, dtype=torch.uint8, device=device),
+            torch.zeros(quant.fp4_scale_tiles(8, 32800, fmt), dtype=torch.uint8, device=device), None, fmt)),
+        "bias of another length": lambda: ops.linear(x, w4, bias=r(32)),
+        "fp32 bias": lambda: ops.linear(x, w4, bias=r(40).float()),
+        "bias with a stride": lambda: ops.linear(x, w4, bias=r(80)[::2]),
+        "fp32 residual": lambda: ops.linear(x, w4, residual=r(4, 40).float()),
+        "residual of fewer rows": lambda: ops.linear(x, w4, residual=r(3, 40)),
+        "residual across": lambda: ops.linear(x, w4, residual=r(40, 4).t()),
+        "out of another width": lambda: ops.linear(x, w4, out=r(4, 32)),
+        "out with rows 44 apart": lambda: ops.linear(x, w4, out=r(4, 44)[:, :40]),
+        "out off 16 bytes": lambda: ops.linear(x, w4, out=buf[:, 4:44]),
+        "out of one row": lambda: ops.linear(x, w4, out=lone.expand(4, 40)),
+        "out with rows that overlap": lambda: ops.linear(x, w4, out=r(200).as_strided((4, 40), (32, 1))),
+        "activation": lambda: ops.linear(x, w4, act="relu"),
+        "factors with a stride": lambda: ops.linear(x, scaled),
+        "scales with a stride": lambda: ops.linear(quant.Fp4Rows(q.q, apart, q.row_scale, fmt), w4),
+        "codes off 16 bytes": lambda: ops.linear(quant.Fp4Rows(codes[:, 8:], q.scale, q.row_scale, fmt), w4),
+        "experts for a layer": lambda: ops.linear(x, e4),
+        "rows of a routing for a layer": lambda: ops.linear(ops.quant_fp4(x, fmt, list2), w4),
+        "a layer for experts": lambda: stream_ops.grouped_linear(x, w4, list2),
+        "a routing of three experts": lambda: stream_ops.grouped_linear(x, e4, routing_of([2, 1, 1], device)),
+        "rows without the routing": lambda: stream_ops.grouped_linear(q, e4, list2),
+        "rows of another routing": lambda: stream_ops.grouped_linear(ops.quant_fp4(x, fmt, routing_of([2, 2], device)),
+                                                                     e4, list2),
+        "experts of another width": lambda: stream_ops.grouped_linear(r(4, 96), e4, list2),
+        "experts: 36 features": lambda: stream_ops.grouped_linear(x, w(2, 36, 64), list2),
+        "experts: 48 gate and up rows": lambda: stream_ops.grouped_linear(x, w(2, 48, 64), list2, "silu"),
+        "expansion into fp32": lambda: ops.dequant_fp4(q, out=torch.empty(4, 64, device=device)),
+        "expansion into another shape": lambda: ops.dequant_fp4(q, out=r(4, 96)),
+        "expansion into a part of a buffer": lambda: ops.dequant_fp4(q, out=r(4, 128)[:, :64]),
     }

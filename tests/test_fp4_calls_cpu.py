@@ -40,3 +40,8 @@ def _all_refused(calls):
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_refused_norms_and_activations(fmt):
     _all_refused(fp4_calls.norm_and_activation("cpu", fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_refused_products(fmt):
+    _all_refused(fp4_calls.products("cpu", fmt))
