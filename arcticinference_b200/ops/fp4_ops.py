@@ -245,7 +245,10 @@ def _grouped_ref(x, w, routing, act):
     v = _ref_rows(x, w, routing)
     _need(N % (32 if act else 8) == 0, "grouped_linear_fp4: N a multiple of %d, got %d", 32 if act else 8, N)
     m = quant.dequantize_fp4_ref(w)
-    y = torch.cat([ve @ m[e].t() for e, ve in enumerate(v.split(routing.counts))])
+    y, first = v.new_zeros(v.shape[0], N), 0
+    for e, count in enumerate(routing.counts):
+        y[first:first + count] = v[first:first + count] @ m[e].t()
+        first += count
     if act is not None:
         v = y.reshape(y.shape[0], N // 32, 2, 16)
         y = act.join(v[:, :, 0], v[:, :, 1]).reshape(y.shape[0], N // 2)

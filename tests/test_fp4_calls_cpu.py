@@ -45,3 +45,14 @@ def test_refused_norms_and_activations(fmt):
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_refused_products(fmt):
     _all_refused(fp4_calls.products("cpu", fmt))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_beyond_a_routing_and_a_routing_beyond_the_rows(fmt):
+    """As with the kernels: what a tile holds and is there is served."""
+    w4 = quant.quantize_weight_fp4(_rand(3, 64, 96, seed=1, scale=0.1), fmt)
+    x, r = _rand(12, 96, seed=2), routing_of([4, 0, 5], "cpu")
+    whole = stream_ops.grouped_linear(x[:9], w4, r)
+    got = stream_ops.grouped_linear(x, w4, r)
+    assert got.shape == (12, 64) and torch.equal(got[:9], whole)
+    assert torch.equal(stream_ops.grouped_linear(x[:6], w4, r), whole[:6])
