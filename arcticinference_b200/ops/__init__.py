@@ -391,6 +391,8 @@ def linear(x: torch.Tensor, w, bias=None, residual=None, act=None, out=None,
         if isinstance(w, Fp4Weight):
             if sync is not None:
                 raise ValueError("cross-rank ordering is not available for 4-bit linears")
+            if force_splits:
+                raise ValueError("4-bit linears split K as they need: force_splits=%r" % force_splits)
             return linear_fp4(x, w, bias, residual, act, out=out)
         if isinstance(w, Fp8RowWeight):
             return linear_fp8_row(x, w, bias, residual, act, out=out, force_splits=force_splits,
@@ -515,6 +517,8 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual=None, ou
     ``quant`` the result is a ``QuantAct`` (e4m3 rows with one scale per token, produced in the
     same pass) for an fp8 linear layer, with ``quant`` "nvfp4" or "mxfp4" ``Fp4Rows`` for a 4-bit one."""
     if isinstance(quant, str):
+        if out is not None:
+            raise ValueError("rmsnorm to 4 bits makes its own rows: no out")
         return rmsnorm_fp4(x, weight, eps, residual, quant)
     if not x.is_cuda:
         y = ref.rmsnorm(x, weight, eps, residual)
@@ -573,6 +577,8 @@ def silu_mul_blocked(x: torch.Tensor, nblk: int = 1, out=None, quant=False):
     ``QuantAct`` of the same values (one scale per token over the whole output row), with ``quant`` "nvfp4" or
     "mxfp4" their ``Fp4Rows``."""
     if isinstance(quant, str):
+        if out is not None:
+            raise ValueError("silu_mul to 4 bits makes its own rows: no out")
         return silu_mul_fp4(x, nblk, quant)
     if not x.is_cuda:
         y = ref.silu_mul_blocked(x, nblk)

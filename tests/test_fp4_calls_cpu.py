@@ -56,3 +56,15 @@ def test_rows_beyond_a_routing_and_a_routing_beyond_the_rows(fmt):
     got = stream_ops.grouped_linear(x, w4, r)
     assert got.shape == (12, 64) and torch.equal(got[:9], whole)
     assert torch.equal(stream_ops.grouped_linear(x[:6], w4, r), whole[:6])
+
+
+def test_arguments_that_would_be_ignored():
+    """A 4-bit layer splits K as it needs, and quantised rows have no place given beforehand."""
+    x, w4 = _rand(4, 64), quant.quantize_weight_fp4(_rand(32, 64), "nvfp4")
+    calls = {
+        "splits": lambda: ops.linear(x, w4, force_splits=2),
+        "out of the norm": lambda: ops.rmsnorm(x, _rand(64), 1e-5, out=torch.empty_like(x), quant="nvfp4"),
+        "out of the activation": lambda: ops.silu_mul_blocked(x, out=_rand(4, 32), quant="mxfp4"),
+    }
+    _all_refused(calls)
+    assert ops.linear(x, w4, force_splits=0).shape == (4, 32)
