@@ -190,6 +190,7 @@ __device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int lane)
 // the unfused kernel adds: 4096 x 4096 17.7 us, 2.4 TB/s, its instructions. SiLU, 4096 x 14336: 58 us, 4.6 TB/s.)
 template <int SRC, bool MX, int VPT, bool WARP>
 __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
+  static_assert(!(WARP && SRC == kFp4Norm), "a norm's sum is the block's");
   pdl_wait();
   pdl_trigger();
   __shared__ uint32_t red[32];
@@ -428,25 +429,27 @@ static int launch_quant_fp4(const QuantFp4Args& a, long long M, cudaStream_t str
   auto go = [&](auto kernel, long long blocks, int threads) {
     return launch_pdl(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, stream, args) == cudaSuccess ? 0 : -5;
   };
-  if (SRC == kFp4Norm) {   // 256 threads: the norm's sum has the order of the unfused kernel's
+  if constexpr (SRC == kFp4Norm) {   // 256 threads: the norm's sum has the order of the unfused kernel's
     if (vecs <= 256) return go(quant_fp4_kernel<SRC, MX, 1, false>, M, 256);
     if (vecs <= 512) return go(quant_fp4_kernel<SRC, MX, 2, false>, M, 256);
     if (vecs <= 1024) return go(quant_fp4_kernel<SRC, MX, 4, false>, M, 256);
     return vecs <= 2048 ? go(quant_fp4_kernel<SRC, MX, 8, false>, M, 256) : -6;
+  } else {
+    // Few rows want many threads each, many rows much in flight per thread (4096 columns, nvfp4, us for 2, 4 and 8
+    // steps: 128 rows 1.75, 1.89, 2.35; 8192 rows 20.2, 17.1, 16.0). The activation holds both factors: 4096 rows
+    // of 14336 62.3 with 4 steps and 110 with 8.
+    const bool many = M >= 148 * 8;
+    if (vecs <= 64) return go(quant_fp4_kernel<SRC, MX, 2, true>, (M + 3) / 4, 128);
+    if (vecs <= 128 && many) return go(quant_fp4_kernel<SRC, MX, 4, true>, (M + 3) / 4, 128);
+    if constexpr (SRC == kFp4Plain)
+      if (vecs <= 256 && many) return go(quant_fp4_kernel<SRC, MX, 8, true>, (M + 3) / 4, 128);
+    int vpt = !many ? 2 : SRC == kFp4Silu ? 4 : 8;
+    while (vecs > 512 * vpt) vpt *= 2;
+    const int threads = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
+    if (vpt == 2) return go(quant_fp4_kernel<SRC, MX, 2, false>, M, threads);
+    if (vpt == 4) return go(quant_fp4_kernel<SRC, MX, 4, false>, M, threads);
+    return vpt == 8 ? go(quant_fp4_kernel<SRC, MX, 8, false>, M, threads) : -6;
   }
-  // Few rows want many threads each, many rows much in flight per thread (4096 columns, nvfp4, us for 2, 4 and 8
-  // steps: 128 rows 1.75, 1.89, 2.35; 8192 rows 20.2, 17.1, 16.0). The activation holds both factors: 4096 rows
-  // of 14336 62.3 with 4 steps and 110 with 8.
-  const bool many = M >= 148 * 8;
-  if (vecs <= 64) return go(quant_fp4_kernel<SRC, MX, 2, true>, (M + 3) / 4, 128);
-  if (vecs <= 128 && many) return go(quant_fp4_kernel<SRC, MX, 4, true>, (M + 3) / 4, 128);
-  if (SRC == kFp4Plain && vecs <= 256 && many) return go(quant_fp4_kernel<SRC, MX, 8, true>, (M + 3) / 4, 128);
-  int vpt = !many ? 2 : SRC == kFp4Silu ? 4 : 8;
-  while (vecs > 512 * vpt) vpt *= 2;
-  const int threads = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
-  if (vpt == 2) return go(quant_fp4_kernel<SRC, MX, 2, false>, M, threads);
-  if (vpt == 4) return go(quant_fp4_kernel<SRC, MX, 4, false>, M, threads);
-  return vpt == 8 ? go(quant_fp4_kernel<SRC, MX, 8, false>, M, threads) : -6;
 }
 
 }  // namespace ab200

@@ -1,6 +1,8 @@
 """How the 4-bit products are launched and what the C entries refuse, without a GPU."""
 
 import ctypes
+import re
+import subprocess
 
 import pytest
 
@@ -60,3 +62,15 @@ def _linear_fp4(M, N, K, gate, act=0, tiles=False):
 def test_a_gate_without_a_list_is_refused(M, gate):
     """Only products of lists join gate and up: others would store N columns where out has N / 2."""
     assert _linear_fp4(M, 256, 512, gate) == -2
+
+
+def test_only_quantisers_that_a_call_reaches_are_built():
+    """Sources 0 (plain), 1 (norm), 2 (activation); vectors a thread; whether a warp has a row. A norm's rows are never a
+    warp's: its sum needs the block."""
+    lib = build.load_kernels()._name
+    names = subprocess.run(["nm", "-C", lib], capture_output=True, text=True, check=True).stdout
+    found = {tuple(t.strip() for t in m.split(",")) for m in re.findall(r"\bquant_fp4_kernel<([^<>]*)>\(", names)}
+    found = {(int(a.split(")")[-1]), int(v), w) for a, _, v, w in found}
+    want = {(1, v, "false") for v in (1, 2, 4, 8)} | {(s, v, "false") for s in (0, 2) for v in (2, 4, 8)} | \
+        {(0, v, "true") for v in (2, 4, 8)} | {(2, v, "true") for v in (2, 4)}
+    assert found == want, (found - want, want - found)
