@@ -1,15 +1,18 @@
 """4-bit kernels where several of their mechanisms meet: K split inside clusters, rings that wrap, lists that say more than
 they hold, factors at the ends of their range."""
 
+import ctypes
+
 import pytest
 import torch
 
-from arcticinference_b200 import ops
+from arcticinference_b200 import build, ops
 from arcticinference_b200.models import quant
 from arcticinference_b200.ops import stream_ops
 
 import fp4_calls
-from fp4_util import FORMATS, oracle_rows, oracle_values, product_bound, routing_of
+from fp4_util import FORMATS, oracle_rows, oracle_values, routing_of
+from test_fp4_gpu import _check
 
 pytestmark = pytest.mark.gpu
 
@@ -186,3 +189,96 @@ def test_refused_norms_and_activations(fmt):
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_refused_products(fmt):
     _all_refused(fp4_calls.products("cuda", fmt))
+
+
+# ------------------------------------------------------------------------ K split inside clusters, and rings that wrap
+def _parts(M, N, K, fmt):
+    P = ctypes.POINTER
+    fn = build.load_kernels().ab200_linear_fp4_plan
+    fn.argtypes = [ctypes.c_longlong] + [ctypes.c_int] * 4 + [P(ctypes.c_int), P(ctypes.c_int), P(ctypes.c_longlong)]
+    parts, columns, smem = ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert fn(M, N, K, FORMATS.index(fmt), sms, parts, columns, smem) == 0
+    return parts.value
+
+
+# (15 steps: parts of 8 and 7, or 4, 4, 4 and 3; 16, 18 and 56; 9 for few tokens: 5 and 4)
+SPLIT = [(M, N, K) for M in (1, 7, 33, 64, 100, 128)
+         for N, K in ((264, 3616), (264, 4096), (520, 4384), (520, 14336), (4096, 4096))] + [(1, 264, 2304), (33, 264, 2304)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", SPLIT)
+def test_split_products(fmt, M, N, K):
+    """The exchange of sums between the CTAs of a cluster, with everything that its epilogue does."""
+    assert _parts(M, N, K, fmt) in (2, 4)
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=K ** -0.5).cuda(), fmt)
+    wd = oracle_values(w4.q, w4.scale, w4.row_scale, fmt).cuda()
+    x, bias, res = _rand(M, K, seed=2), _rand(N, seed=3), _rand(M, N, seed=4)
+    _check(x, w4, fmt, wd=wd)
+    _check(x, w4, fmt, bias=bias, wd=wd)
+    _check(x, w4, fmt, bias=bias, act="gelu", wd=wd)
+    _check(x, w4, fmt, residual=res, wd=wd)
+    want = _check(x, w4, fmt, bias=bias, act="gelu", residual=res, wd=wd)
+    place = res.cuda()
+    got = ops.linear(x.cuda(), w4, bias=bias.cuda(), act="gelu", residual=place, out=place)
+    assert got is place and torch.equal(got, want)
+    buf = torch.full((M + 2, N + 24), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.linear(x.cuda(), w4, bias=bias.cuda(), act="gelu", residual=res.cuda(), out=buf[1:M + 1, 8:N + 8])
+    assert torch.equal(buf[1:M + 1, 8:N + 8], want)
+    buf[1:M + 1, 8:N + 8] = 5.0
+    assert bool((buf == 5).all())
+    ops.check_status()
+
+
+def test_split_products_have_both_numbers_of_parts():
+    assert {_parts(M, N, K, fmt) for fmt in FORMATS for M, N, K in SPLIT} == {2, 4}
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [1, 70, 128])
+def test_two_ctas_an_sm_whose_rings_wrap(fmt, M):
+    """More tiles than SMs, and more steps than stages."""
+    N, K = 19208, 4128
+    assert _parts(M, N, K, fmt) == 1
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=K ** -0.5).cuda(), fmt)
+    x, res = _rand(M, K, seed=2), _rand(M, N, seed=4)
+    wd = oracle_values(w4.q, w4.scale, w4.row_scale, fmt).cuda()
+    _check(x, w4, fmt, wd=wd)
+    _check(x, w4, fmt, residual=res, bias=_rand(N, seed=3), wd=wd)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 520, 4096), (33, 4096, 4096), (128, 264, 2304), (100, 520, 512), (150, 520, 1056),
+                                   (400, 520, 1056), (1000, 520, 1056)])
+def test_a_row_gets_the_same_bits_wherever_it_stands(fmt, M, N, K):
+    """Every run, and every order of a batch's rows."""
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=0.1).cuda(), fmt)
+    x = _rand(M, K, seed=2).cuda()
+    first = ops.linear(x, w4)
+    for i in range(4):
+        order = torch.randperm(M, generator=torch.Generator().manual_seed(i)).cuda()
+        assert torch.equal(ops.linear(x, w4), first)
+        assert torch.equal(ops.linear(x[order], w4), first[order])
+
+
+def test_every_scale_of_e4m3():
+    """All 126 positive e4m3 numbers as block scales, each with values around every border of e2m1 in its units; and the
+    largest values of a block around the borders between two scales."""
+    scales = torch.arange(1, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    rows = []
+    for s in scales.tolist():
+        v = (borders[:, None] * torch.tensor([1 - 2.0 ** -7, 1.0, 1 + 2.0 ** -7])[None]).flatten() * s
+        top = torch.full((1,), 6 * s)
+        rows.append(torch.cat([top, v[:15], top, v[6:], torch.full((32,), 2688.0)]))
+    both = (scales[:-1] + scales[1:]) / 2 * 6
+    for b in both.tolist():
+        for f in (1 - 2.0 ** -7, 1.0, 1 + 2.0 ** -7):
+            rows.append(torch.cat([torch.full((32,), b * f), torch.full((32,), 2688.0)]))
+    x = torch.stack(rows).to(torch.bfloat16)
+    a = ops.quant_fp4(x.cuda(), "nvfp4")
+    assert torch.equal(a.row_scale.cpu(), torch.ones(len(rows)))
+    byte = quant.untile_fp4_scales(a.scale, len(rows), 4).cpu()
+    assert set(byte[:126, 0].tolist()) == set(range(1, 127))
+    assert torch.equal(oracle_values(a.q, a.scale, a.row_scale, "nvfp4"), oracle_rows(x, "nvfp4"))
