@@ -80,8 +80,8 @@ def quant_fp4(x: torch.Tensor, fmt: str = "nvfp4", routing=None):
 
 
 def dequant_fp4(rows, out: torch.Tensor = None) -> torch.Tensor:
-    """The bf16 numbers that ``rows`` (``Fp4Rows`` or ``Fp4Weight``) stand for, each rounded once; exact where the row
-    factors are powers of two, as the quantisers' are. With a routing, rows that no tile holds are not written."""
+    """The bf16 numbers that ``rows`` (``Fp4Rows`` or ``Fp4Weight``) stand for: block scale times row factor and that times the
+    code, each rounded to fp32, then to bf16. Exact where the factors are powers of two, as the quantisers' are. With a routing, rows that no tile holds are not written."""
     if not rows.is_cuda:
         from ..models import quant
         plain = rows if rows.routing is None else quant.Fp4Rows(rows.q, rows.scale, rows.row_scale, rows.fmt)

@@ -282,3 +282,22 @@ def test_every_scale_of_e4m3():
     byte = quant.untile_fp4_scales(a.scale, len(rows), 4).cpu()
     assert set(byte[:126, 0].tolist()) == set(range(1, 127))
     assert torch.equal(oracle_values(a.q, a.scale, a.row_scale, "nvfp4"), oracle_rows(x, "nvfp4"))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_expansion_with_any_factors(fmt):
+    """The same bits as on the CPU, also where a factor is no power of two and rounds on the way (8 million numbers: the
+    other order of the two products changes 700000 of them in fp32)."""
+    R, K = 2000, 4096
+    gen = torch.Generator().manual_seed(2)
+    q = torch.randint(0, 256, (R, K // 2), generator=gen, dtype=torch.uint8)
+    low, high = (40, 72) if fmt == "nvfp4" else (120, 134)
+    scale = torch.randint(low, high, quant.fp4_scale_tiles(R, K, fmt), generator=gen, dtype=torch.uint8)
+    g = torch.rand(R, generator=gen) + 0.3
+    g[::7] *= 2.0 ** -110
+    g[1::7] *= 2.0 ** 100
+    want = quant.Fp4Weight(q, scale, g, fmt).dequantize()
+    got = quant.Fp4Weight(q.cuda(), scale.cuda(), g.cuda(), fmt).dequantize().cpu()
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+    v = oracle_values(q[:200], scale[:2], g[:200], fmt)          # bf16's rounding and two of fp32's
+    assert ((got[:200].double() - v).abs() <= (2.0 ** -8 + 2.0 ** -22) * v.abs()).all()
