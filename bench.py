@@ -42,7 +42,7 @@ def parse_args():
     ap.add_argument("--impl", type=str, default="ours", choices=["ours", "reference"])
     ap.add_argument("--model", type=str, default="llama-3.1-8b")
     ap.add_argument("--quantization", type=str, default="fp8",
-                    help='"fp8" (block-scaled fp8 weights, bf16 activations; the named config) or "none" (bf16)')
+                    help='"fp8" (fp8 weights, bf16 activations; the named config), "nvfp4", "mxfp4" or "none" (bf16)')
     ap.add_argument("--requests-per-gpu", type=int, default=128)
     ap.add_argument("--input-len", type=int, default=2000)
     ap.add_argument("--output-len", type=int, default=250)
@@ -229,6 +229,11 @@ def run_reference(args, rank, local_rank):
     return 0
 
 
+def compute_type(quant) -> str:
+    """The ``dtype`` of the line, by the quantisation of the linear layers."""
+    return "%s-weights/bf16-activations" % quant if quant else "bf16"
+
+
 def main():
     args = parse_args()
     rank = int(os.environ.get("RANK", "0"))
@@ -343,7 +348,7 @@ def main():
             "value": value, "unit": "tokens/s", "n_gpus": n_gpus, "steps": args.steps,
             "warmup": args.warmup, "ms_per_step": dev_ms / args.steps,
             "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-            "dtype": "bf16" if not quant else "fp8-weights/bf16-activations",
+            "dtype": compute_type(quant),
             "data": "synthetic (uniform-random token ids, random-init weights)",
             "p50_ttft_ms": 1000 * statistics.median(ttfts) if ttfts else None,
             "p50_tpot_ms": 1000 * statistics.median(tpots) if tpots else None,

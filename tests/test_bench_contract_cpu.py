@@ -15,3 +15,10 @@ def test_reference_arm_reports_unavailable():
     line = [l for l in p.stdout.splitlines() if l.startswith("{")][-1]
     d = json.loads(line)
     assert d["impl"] == "reference" and isinstance(d["unavailable"], str) and d["unavailable"]
+
+
+def test_the_line_names_the_type_of_the_linears():
+    sys.path.insert(0, REPO)
+    import bench
+    assert bench.compute_type(None) == "bf16" and bench.compute_type("fp8") == "fp8-weights/bf16-activations"
+    assert bench.compute_type("nvfp4").startswith("nvfp4-") and bench.compute_type("mxfp4").startswith("mxfp4-")
