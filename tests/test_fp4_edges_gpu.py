@@ -301,3 +301,29 @@ def test_expansion_with_any_factors(fmt):
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
     v = oracle_values(q[:200], scale[:2], g[:200], fmt)          # bf16's rounding and two of fp32's
     assert ((got[:200].double() - v).abs() <= (2.0 ** -8 + 2.0 ** -22) * v.abs()).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,inter,nblk", [(3, 40, 4), (1300, 8, 4), (130, 72, 12), (2, 24, 1364)])
+def test_blocks_of_the_activation_that_end_inside_a_piece(fmt, M, inter, nblk):
+    """A thread's 16 columns then belong to two (gate | up) blocks."""
+    x = _rand(M, 2 * inter * nblk, seed=inter).cuda()
+    a, b = ops.silu_mul_blocked(x, nblk, quant=fmt), ops.quant_fp4(ops.silu_mul_blocked(x, nblk), fmt)
+    assert torch.equal(a.dequantize(), b.dequantize())
+    want = oracle_rows(ops.silu_mul_blocked(x, nblk).cpu(), fmt)
+    assert torch.equal(a.dequantize().cpu(), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_and_weights_that_are_parts_of_larger_ones(fmt):
+    """Codes whose rows lie apart, of the rows and of the weight."""
+    M, N, K = 70, 136, 256
+    w4 = quant.quantize_weight_fp4(_rand(N, K, seed=1, scale=0.1).cuda(), fmt)
+    q = ops.quant_fp4(_rand(M, K, seed=2).cuda(), fmt)
+    want = ops.linear(q, w4)
+    apart = lambda t: torch.cat([t, torch.full_like(t, 255)], 1)[:, :t.shape[1]]
+    x2, w2 = quant.Fp4Rows(apart(q.q), q.scale, q.row_scale, fmt), quant.Fp4Weight(apart(w4.q), w4.scale, w4.row_scale, fmt)
+    assert x2.q.stride(0) == K and w2.q.stride(0) == K
+    assert torch.equal(ops.linear(x2, w2), want) and torch.equal(x2.dequantize(), q.dequantize())
+    x3 = quant.Fp4Rows(apart(q.q[:1]), q.scale, None if q.row_scale is None else q.row_scale[:1], fmt)
+    assert torch.equal(ops.linear(x3, w2), ops.linear(ops.quant_fp4(_rand(M, K, seed=2)[:1].cuda(), fmt), w4))
