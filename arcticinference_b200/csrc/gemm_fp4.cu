@@ -11,9 +11,10 @@
 // scales to tensor memory (sets used in turn) and issues the products into one of two accumulators;
 // eight warps drain the other one.
 //
-// One B200, nvfp4: 8192 x 28672 x 4096 370 to 380 us (5.1 to 5.2 PFLOP/s; mxfp4 343 to 352, 5.5 to 5.6), bound by shared memory
-// (608 cycles of copies and operands per 512 of products); 49152 rows of 64 experts, 2 x 1408 from 2048, 149 to 154 us, bound
-// by the boundaries of tiles of eight steps; 768 rows 39 us, the weights at 5.3 TB/s.
+// One B200, nvfp4: 8192 x 28672 x 4096 375 to 383 us (5.0 to 5.1 PFLOP/s; mxfp4 354 to 366, 5.3 to 5.4), bound by shared memory
+// (608 cycles of copies and operands per 512 of products); 49152 rows of 64 experts, 2 x 1408 from 2048, 148 to 153 us, bound
+// by the boundaries of tiles of eight steps; 768 rows 39 us, the weights at 5.4 TB/s. (Lists run in pairs from 640 rows an
+// expert on, a border that the router took from bf16 products; in 4 bits the two forms have not been compared.)
 
 #include <string.h>
 
@@ -626,8 +627,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 // the sender's shared memory first and from there as bulk copies that complete on a barrier of the receiver; stores
 // into another CTA's memory, eight bytes a lane, and a cluster barrier on either side took 5.5 us for 128 tokens. The
 // weights' first steps are requested into L2 before the wait for the kernel ahead, whose tail (the rows' quantisation)
-// they cover: a prefetch changes no value, whoever has written them. One token, nvfp4: 28672 x 4096 12.9 us (5.1 TB/s),
-// 4096 x 14336 10.4 us (3.2; 25.4 before K was split), 4096 x 4096 5.2 us; 128 tokens 15.2, 12.7 and 7.9 us.
+// they cover: a prefetch changes no value, whoever has written them. One token, nvfp4: 28672 x 4096 13.0 us (5.1 TB/s),
+// 4096 x 14336 10.6 us (3.1; 25.4 before K was split), 4096 x 4096 5.5 us; 128 tokens 15.5, 12.9 and 8.1 us.
 struct Fp4FewArgs {
   int N, M, kblocks, splits, per_split, stages;
   uint32_t b_bytes, columns, scale_at, recv_at;
@@ -644,7 +645,8 @@ struct Fp4FewArgs {
 
 constexpr int kFewSlice = 16;                    // features of an exchanged slice
 constexpr uint32_t kFewHeader = 1024;            // barriers in front of the stages
-// Tensor memory: the accumulator, then a set of scales per stage, so that a stage's wait covers its set too.
+// Tensor memory: the accumulator, then a set of scales per stage, so that a stage's wait covers its set too. (A CTA of a
+// cluster takes at most 256 columns: fp4_few_plan.)
 constexpr uint32_t kFewScaleSet = 32;
 constexpr int kFewTokens = 128;
 

@@ -186,8 +186,10 @@ __device__ __forceinline__ int fq_slot(const QuantFp4Args& p, int row, int lane)
 
 // WARP: a warp per row and no barrier, for rows that 32 threads hold; otherwise a block per row. A thread takes pieces
 // of 16 columns, whose one scale (nvfp4) it then computes alone: 8192 x 4096 took 16.1 us with pieces of 8, and the
-// instructions bound it; with pieces of 16 it takes 14.5 (5.9 TB/s; mxfp4 13.3, 6.4). (The norm keeps pieces of 8, in which
-// the unfused kernel adds: 4096 x 4096 17.7 us, 2.4 TB/s, its instructions. SiLU, 4096 x 14336: 58 us, 4.6 TB/s.)
+// instructions bound it; with pieces of 16 it takes 14.5 (5.9 TB/s; mxfp4 13.3, 6.4). (The norm keeps
+// pieces of 8, in which the unfused kernel adds; both lanes of an nvfp4 block then compute its scale. That order binds the
+// sum only, and pieces of 16 behind it have not been tried: 4096 x 4096 17.8 us, 2.4 TB/s, an instruction issued in 78 % of
+// the cycles. SiLU, 4096 x 14336: 58 us, 4.6 TB/s, 67 %.)
 template <int SRC, bool MX, int VPT, bool WARP>
 __global__ void __launch_bounds__(512) quant_fp4_kernel(const QuantFp4Args p) {
   static_assert(!(WARP && SRC == kFp4Norm), "a norm's sum is the block's");
