@@ -481,6 +481,21 @@ at::Tensor fp4_dequant(const at::Tensor& q, const at::Tensor& scale, const OptTe
   return out;
 }
 
+// Whether two matrices of bf16 rows share an element, other than all of them in the same places: the CTA that stores
+// it and the one that reads it do not wait for one another.
+bool fp4_shares(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t M = a.size(0), width = a.size(1);
+  if (M == 0 || width == 0) return false;
+  auto from = [](const at::Tensor& t) { return reinterpret_cast<intptr_t>(t.data_ptr()) / 2; };
+  const int64_t sa = M > 1 ? a.stride(0) : width, sb = M > 1 ? b.stride(0) : width;
+  const int64_t apart = from(a) - from(b);
+  if (apart == 0 && sa == sb) return false;
+  if (apart >= (M - 1) * sb + width || -apart >= (M - 1) * sa + width) return false;
+  if (sa != sb || sa < width) return true;
+  const int64_t in = (apart % sa + sa) % sa;      // columns of equal pitch, beside one another
+  return in < width || sa - in < width;
+}
+
 // x: bf16 rows, quantised here into scratch, or xq, xs, xg
 void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, const OptTensor& xg,
                  const at::Tensor& wq, const at::Tensor& ws, const OptTensor& wg, int64_t fmt, const OptTensor& bias,
@@ -533,6 +548,7 @@ void fp4_product(const OptTensor& x0, const OptTensor& xq, const OptTensor& xs, 
   if (out.defined()) {
     matrix(out, "out");
     TORCH_CHECK_VALUE(M <= 1 || out.stride(0) >= width, "4-bit product: rows of out overlap");
+    TORCH_CHECK_VALUE(!has(residual) || !fp4_shares(*residual, out), "4-bit product: out overlaps residual");
   }
   else out = at::empty({M, width}, wq.options().dtype(at::kBFloat16));
   if (M == 0 || N == 0) return;

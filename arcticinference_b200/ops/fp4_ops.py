@@ -150,7 +150,7 @@ def _operand(x, w, routing=None):
 def linear_fp4(x, w, bias=None, residual=None, act=None, out=None) -> torch.Tensor:
     """``out = act(x @ w.T + bias) + residual`` with both operands in 4 bits: ``x`` bf16 [M, K] (quantised here) or
     ``Fp4Rows``, ``w`` an ``Fp4Weight`` [N, K] with N a multiple of 8. Sums are fp32, the result is rounded once to bf16.
-    ``out`` may be ``residual``."""
+    ``out`` may be ``residual``, or has no element of it."""
     code = _ACT.get(act)
     _need(code is not None, "linear_fp4: activation %r", act)
     wq = getattr(w, "q", None)
@@ -197,6 +197,20 @@ def _ref_rows(x, w, routing=None):
     return quant.dequantize_fp4_ref(quant_fp4(x, w.fmt))
 
 
+def _shares(a, b) -> bool:
+    """Whether two matrices of bf16 rows share an element, other than all of them in the same places."""
+    M, width = a.shape
+    if M == 0 or width == 0:
+        return False
+    sa, sb = (a.stride(0), b.stride(0)) if M > 1 else (width, width)
+    apart = (a.data_ptr() - b.data_ptr()) // 2
+    if apart == 0 and sa == sb or apart >= (M - 1) * sb + width or -apart >= (M - 1) * sa + width:
+        return False
+    if sa != sb or sa < width:
+        return True
+    return apart % sa < width or sa - apart % sa < width      # columns of equal pitch, beside one another
+
+
 def _linear_ref(x, w, bias, residual, act, out):
     from ..models import quant
     N = w.shape[0]
@@ -209,6 +223,7 @@ def _linear_ref(x, w, bias, residual, act, out):
             _lies(t, t.is_contiguous() if name == "bias" else
                   t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0, name)
     _need(out is None or M <= 1 or out.stride(0) >= N, "4-bit product: rows of out overlap")
+    _need(out is None or residual is None or not _shares(residual, out), "4-bit product: out overlaps residual")
     y = v @ quant.dequantize_fp4_ref(w).t()
     if bias is not None:
         y = y + bias.float()

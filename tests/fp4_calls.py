@@ -84,3 +84,31 @@ def products(device, fmt):
         "expansion into another shape": lambda: ops.dequant_fp4(q, out=r(4, 96)),
         "expansion into a part of a buffer": lambda: ops.dequant_fp4(q, out=r(4, 128)[:, :64]),
     }
+
+
+def overlaps(device, fmt):
+    """A residual that shares elements with the output, but not all of them in the same places."""
+    r = lambda *s: _rand(*s, device=device)
+    w4, x, buf = quant.quantize_weight_fp4(r(40, 64), fmt), r(4, 64), r(6, 96)
+    long = r(400)
+    return {
+        "a row above": lambda: ops.linear(x, w4, residual=buf[:4, :40], out=buf[1:5, :40]),
+        "eight columns on": lambda: ops.linear(x, w4, residual=buf[:4, :40], out=buf[:4, 8:48]),
+        "another distance of rows": lambda: ops.linear(x, w4, residual=long.as_strided((4, 40), (40, 1)),
+                                                       out=long.as_strided((4, 40), (48, 1))),
+        "one row for all, in the output": lambda: ops.linear(x, w4, residual=buf[:1, :40].expand(4, 40), out=buf[:4, :40]),
+    }
+
+
+def no_overlaps(device, fmt):
+    """(call, the same with a residual of its own): parts of one buffer that share nothing, and the output itself."""
+    r = lambda *s: _rand(*s, device=device)
+    w4, x = quant.quantize_weight_fp4(r(40, 64), fmt), r(4, 64)
+    out = []
+    for res, to in ((lambda b: b[:4, :40], lambda b: b[:4, 48:88]), (lambda b: b[:4, 48:88], lambda b: b[:4, :40]),
+                    (lambda b: b[:4, :40], lambda b: b[4:8, :40]), (lambda b: b[:4, 8:48], lambda b: b[:4, 8:48]),
+                    (lambda b: b[4:5, :40].expand(4, 40), lambda b: b[:4, :40])):
+        buf = r(9, 96)
+        out.append((lambda b=buf, f=res, g=to: ops.linear(x, w4, residual=f(b), out=g(b)),
+                    lambda b=buf.clone(), f=res: ops.linear(x, w4, residual=f(b).contiguous())))
+    return out

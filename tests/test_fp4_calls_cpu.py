@@ -68,3 +68,11 @@ def test_arguments_that_would_be_ignored():
     }
     _all_refused(calls)
     assert ops.linear(x, w4, force_splits=0).shape == (4, 32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_residuals_that_overlap_the_output(fmt):
+    _all_refused(fp4_calls.overlaps("cpu", fmt))
+    for call, apart in fp4_calls.no_overlaps("cpu", fmt):
+        want = apart()
+        assert torch.equal(call(), want)

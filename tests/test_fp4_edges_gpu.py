@@ -327,3 +327,11 @@ def test_rows_and_weights_that_are_parts_of_larger_ones(fmt):
     assert torch.equal(ops.linear(x2, w2), want) and torch.equal(x2.dequantize(), q.dequantize())
     x3 = quant.Fp4Rows(apart(q.q[:1]), q.scale, None if q.row_scale is None else q.row_scale[:1], fmt)
     assert torch.equal(ops.linear(x3, w2), ops.linear(ops.quant_fp4(_rand(M, K, seed=2)[:1].cuda(), fmt), w4))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_residuals_that_overlap_the_output(fmt):
+    _all_refused(fp4_calls.overlaps("cuda", fmt))
+    for call, apart in fp4_calls.no_overlaps("cuda", fmt):
+        want = apart()
+        assert torch.equal(call(), want)
